@@ -199,6 +199,93 @@ int gs_fused_adam_slab(float* theta, const float* g, float* m, float* v, const i
                        const float* grad_bias_host, int g_cols, int count_col, const float* count_coef_host,
                        int row_select, gs_stream_t stream);
 
+/* ------------------------------------------------------------------ AdamW over many tensors */
+
+/* Element types of tensors and moments. */
+#define GS_F32 0
+#define GS_BF16 1
+#define GS_F16 2
+
+/* Elements of a tensor that share one exponent in the 8-bit form of the moments. */
+#define GS_MOMENT_BLOCK 256
+
+/* One tensor of a call over many.  Element i lies at row i / cols, column
+ * i % cols; rows are ``*_stride`` elements apart (a dense tensor: cols = n, or
+ * a stride equal to cols).  ``param`` is what a call updates or writes, ``grad``
+ * what it reads.  The table of tensors is passed to the kernels by value: the
+ * caller's array is free again when the call returns. */
+typedef struct gs_tensor {
+    void* param;
+    const void* grad;
+    int64_t n;             /* elements; 0: the tensor is skipped */
+    int64_t state;         /* first element in the state's slabs, a multiple of GS_MOMENT_BLOCK */
+    int64_t cols;
+    int64_t param_stride, grad_stride;
+    int32_t param_type, grad_type;
+    double lr_scale;       /* multiplies the learning rate */
+    double decay;          /* weight decay (decoupled) */
+} gs_tensor;
+
+/* The state of an optimizer: slabs over the elements of all tensors, each
+ * tensor's part starting at its ``state`` offset and padded to whole blocks of
+ * GS_MOMENT_BLOCK elements.  bits = 32: m and v are float32.  bits = 8: they are
+ * codes of one byte, and m_exp/v_exp hold one exponent byte per block; zeroed
+ * buffers are zero moments.  Buffers are 16-byte aligned. */
+typedef struct gs_adamw_state {
+    void *m, *v;
+    uint8_t *m_exp, *v_exp;
+    float* master;         /* optional float32 copies of 16-bit parameters (a slab like m): the update is
+                              applied to them and the parameters are their rounding */
+    int64_t* control;      /* 2 values on the device, zeroed at first: the steps taken, and a counter of the kernel */
+    int32_t bits;
+} gs_adamw_state;
+
+typedef struct gs_adamw_settings {
+    double lr, beta1, beta2;
+    float eps;
+    double grad_scale;            /* multiplies every gradient */
+    const float* lr_device;       /* optional: one float32 on the device that replaces lr */
+    const double* norm_partials;  /* optional, from gs_grad_norm_partials over the same gradients: the step clips
+                                     them to max_norm (INFINITY: no clipping) and is skipped as a whole, its count
+                                     included, when the norm is not finite in float32 */
+    int64_t num_partials;
+    double max_norm;
+    float* norm_out;              /* optional: |grad_scale| * norm */
+} gs_adamw_settings;
+
+/* One AdamW step over all tensors: with c = grad_scale, times max_norm / norm
+ * when clipped, and t the new step count,
+ *   g = c * grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+ *   param = (1 - lr decay) param - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ * in float32, every operation rounded by itself; 16-bit parameters (or their
+ * master's rounding) are rounded to nearest at the end.  Values that are not
+ * finite pass into the elements they touch (8-bit moments: into their block).
+ * The step count lives in ``control``, so a captured call can be replayed. */
+int gs_adamw_step(const gs_tensor* tensors, int64_t count, const gs_adamw_state* state,
+                  const gs_adamw_settings* settings, gs_stream_t stream);
+
+/* Partial sums, in float64, of the squares of every tensor's ``grad``; their
+ * number, at most gs_grad_norm_max_partials(count), is returned through the
+ * host pointer ``num_partials``. */
+int64_t gs_grad_norm_max_partials(int64_t count);
+int gs_grad_norm_partials(const gs_tensor* tensors, int64_t count, double* partials, int64_t capacity,
+                          int64_t* num_partials, gs_stream_t stream);
+
+/* param = grad * max_norm / norm when the norm that the partial sums give exceeds
+ * max_norm, else param = grad (nothing is written where they are the same memory);
+ * a norm that is not finite in float32 scales nothing.  norm_out (optional): the norm before. */
+int gs_clip_gradients(const gs_tensor* tensors, int64_t count, const double* partials, int64_t num_partials,
+                      double max_norm, float* norm_out, gs_stream_t stream);
+
+/* Moments to the 8-bit form: ``param`` holds a tensor's m and ``grad`` its v (read
+ * only, any type); ``step`` selects the rounding offsets.  Values that the form can
+ * hold are kept exactly.  And back: whole slabs of n elements to GS_F32 or GS_BF16,
+ * which hold every value of the form exactly. */
+int gs_moments8_quantize(const gs_tensor* tensors, int64_t count, uint8_t* m, uint8_t* v, uint8_t* m_exp,
+                         uint8_t* v_exp, int64_t step, gs_stream_t stream);
+int gs_moments8_dequantize(const uint8_t* m, const uint8_t* v, const uint8_t* m_exp, const uint8_t* v_exp, int64_t n,
+                           int out_type, void* m_out, void* v_out, gs_stream_t stream);
+
 /* ------------------------------------------------------------------ cull */
 
 /* frustum_culling_mlx (mlx_gsplat/rendering.py:41-94): writes the ascending

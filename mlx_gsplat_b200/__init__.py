@@ -6,6 +6,7 @@ Importing the package needs no GPU; every compute call goes to
 ``libgsplat_b200.so`` (built by ``python -m mlx_gsplat_b200.build``) and
 fails loudly without it.
 """
+from .adamw import FusedAdamW, clip_gradients
 from .allocator import PointerStableChunkedAllocator
 from .dataset import Dataset, Parser
 from .optimizer import FusedMLXAdam
@@ -14,6 +15,8 @@ from .rendering import RasterSettings, bilinear_resize_mlx, frustum_culling_mlx,
 __all__ = [
     "PointerStableChunkedAllocator",
     "FusedMLXAdam",
+    "FusedAdamW",
+    "clip_gradients",
     "frustum_culling_mlx",
     "rasterize_gaussians_mlx",
     "bilinear_resize_mlx",

@@ -19,6 +19,8 @@ GS_ADAM_FUSED, GS_ADAM_PURE, GS_ADAM_EXACT = 0, 1, 0x100
 GS_LOSS_NONE, GS_LOSS_L1_U8, GS_LOSS_L1_F32, GS_LOSS_MEAN = 0, 1, 2, 3
 GS_SH_REFERENCE, GS_SH_FULL = 0, 1
 GS_ROWS_ALL, GS_ROWS_SEEN, GS_ROWS_UNSEEN = 0, 1, 2
+GS_F32, GS_BF16, GS_F16 = 0, 1, 2
+GS_MOMENT_BLOCK = 256
 
 c_float_p = ctypes.POINTER(ctypes.c_float)
 c_vp = ctypes.c_void_p
@@ -54,6 +56,17 @@ class GsCamera(ctypes.Structure):
 
 class GsRasterSettings(ctypes.Structure):
     _fields_ = [("alpha_cutoff", ctypes.c_float), ("transmittance_min", ctypes.c_float), ("alpha_mask", i32)]
+
+
+class GsAdamWState(ctypes.Structure):
+    _fields_ = [("m", c_vp), ("v", c_vp), ("m_exp", c_vp), ("v_exp", c_vp), ("master", c_vp), ("control", c_vp),
+                ("bits", i32)]
+
+
+class GsAdamWSettings(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_float), ("grad_scale", ctypes.c_double), ("lr_device", c_vp),
+                ("norm_partials", c_vp), ("num_partials", i64), ("max_norm", ctypes.c_double), ("norm_out", c_vp)]
 
 
 _SIGS = {
@@ -125,6 +138,13 @@ _SIGS = {
     "gs_fill_rows": (ctypes.c_int, [c_vp, i64, i64, c_float_p, c_vp]),
     "gs_fill_column": (ctypes.c_int, [c_vp, i64, i64, ctypes.c_int, ctypes.c_float, c_vp]),
     "gs_mark_slots": (ctypes.c_int, [c_vp, i64, c_vp, i64, ctypes.c_int, c_vp]),
+    # many-tensor calls: the first argument is the address of an array of gs_tensor
+    "gs_adamw_step": (ctypes.c_int, [c_vp, i64, ctypes.POINTER(GsAdamWState), ctypes.POINTER(GsAdamWSettings), c_vp]),
+    "gs_grad_norm_max_partials": (i64, [i64]),
+    "gs_grad_norm_partials": (ctypes.c_int, [c_vp, i64, c_vp, i64, ctypes.POINTER(i64), c_vp]),
+    "gs_clip_gradients": (ctypes.c_int, [c_vp, i64, c_vp, i64, ctypes.c_double, c_vp, c_vp]),
+    "gs_moments8_quantize": (ctypes.c_int, [c_vp, i64, c_vp, c_vp, c_vp, c_vp, i64, c_vp]),
+    "gs_moments8_dequantize": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, i64, ctypes.c_int, c_vp, c_vp, c_vp]),
     "gs_copy_rows": (ctypes.c_int, [c_vp, i64, c_vp, c_vp, i64, c_vp, i64, ctypes.c_int, c_vp]),
 }
 

@@ -1,0 +1,565 @@
+"""AdamW over many separate tensors on B200: ``FusedAdamW`` and ``clip_gradients``.
+
+``FusedMLXAdam`` updates the pooled Gaussian slabs of the trainer; a program
+that trains a scene through autograd (``rasterize_gaussians_mlx`` on leaf
+tensors, or slab views of a pool) with other parameters beside it (appearance
+embeddings, pose deltas, exposure, a small network) has a list of tensors of
+all sizes instead.  ``FusedAdamW`` steps all of them in one launch:
+
+* decoupled weight decay, per-tensor learning-rate and decay factors;
+* parameters and gradients in float32, bfloat16 or float16, optionally with
+  float32 master copies of the 16-bit parameters;
+* moments in 32 bits, or in 8 (``state_bits=8``: 2.02 bytes a parameter instead
+  of 8), rounded without bias over steps, ``moments8.cuh``;
+* clipping by the global gradient norm inside the step (``max_norm``), and
+  skipping of a step whose gradients are not all finite, without a host sync;
+* the step count on the device, so that ``step`` can be captured into a CUDA
+  graph and replayed (``lr`` may be a device tensor).
+
+``clip_gradients`` clips a set of gradients on its own, for other optimizers.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from operator import attrgetter
+from typing import Dict, List, Optional, Sequence, Tuple, Union
+
+import numpy as np
+import torch
+
+from . import _lib
+
+TYPES = {torch.float32: _lib.GS_F32, torch.bfloat16: _lib.GS_BF16, torch.float16: _lib.GS_F16}
+BLOCK = _lib.GS_MOMENT_BLOCK
+_ENTRY = np.dtype([("param", np.uint64), ("grad", np.uint64), ("n", np.int64), ("state", np.int64),
+                   ("cols", np.int64), ("param_stride", np.int64), ("grad_stride", np.int64),
+                   ("param_type", np.int32), ("grad_type", np.int32), ("lr_scale", np.float64),
+                   ("decay", np.float64)], align=True)
+_data_ptr = torch.Tensor.data_ptr
+_is_contiguous = torch.Tensor.is_contiguous
+_device_index = torch.Tensor.get_device
+_dtype = attrgetter("dtype")
+_shape = attrgetter("shape")
+
+
+def rows_of(t: torch.Tensor) -> Optional[Tuple[int, int]]:
+    """``(cols, stride)`` of a tensor whose elements, in order, are rows of
+    ``cols`` adjacent ones ``stride`` apart (``(n, n)`` when it is dense), or
+    None when it has no such form (transposed, broadcast, two strides)."""
+    n = t.numel()
+    if t.is_contiguous():
+        return max(n, 1), max(n, 1)
+    dims = [(s, d) for s, d in zip(t.stride(), t.shape) if d != 1]
+    cols = 1
+    while dims and dims[-1][0] == cols:
+        cols *= dims.pop()[1]
+    if not dims:
+        return n, n
+    stride, rows = dims.pop()
+    if stride < cols:
+        return None
+    reach = stride * rows
+    while dims:
+        s, d = dims.pop()
+        if s != reach:
+            return None
+        reach *= d
+    return cols, stride
+
+
+def _span(t: torch.Tensor, rows: Tuple[int, int]) -> Tuple[int, int]:
+    cols, stride = rows
+    last = (t.numel() // cols - 1) * stride + cols
+    return t.data_ptr(), t.data_ptr() + last * t.element_size()
+
+
+def overlapping(tensors: Sequence[torch.Tensor], rows: Sequence[Tuple[int, int]]) -> Optional[Tuple[int, int]]:
+    """Two of the tensors that share an element, or None.  Columns of one slab
+    interleave without sharing; what cannot be told apart counts as shared."""
+    items = sorted(((*_span(t, r), k) for k, (t, r) in enumerate(zip(tensors, rows)) if t.numel()))
+    group: List[Tuple[int, int, int]] = []
+    reach = -1
+    for lo, hi, k in items:
+        if lo >= reach:
+            group = []
+        for lo2, hi2, j in group:
+            if hi2 <= lo:
+                continue
+            # two sets of rows share nothing when their columns lie apart modulo a distance that divides both pitches
+            (cj, sj), (ck, sk) = rows[j], rows[k]
+            bj, bk = tensors[j].element_size(), tensors[k].element_size()
+            pitch = math.gcd(sj * bj, sk * bk)
+            at = (lo - lo2) % pitch
+            if not (sj > cj and sk > ck and cj * bj <= at and at + ck * bk <= pitch):
+                return j, k
+        group.append((lo, hi, k))
+        reach = max(reach, hi)
+    return None
+
+
+def _check_tensor(what: str, t) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
+    if t.layout != torch.strided:
+        raise ValueError(f"{what}: sparse tensors are not supported")
+    if t.dtype not in TYPES:
+        raise ValueError(f"{what}: {t.dtype} is not float32, bfloat16 or float16")
+
+
+def _check_cuda(tensors: Sequence[torch.Tensor]) -> torch.device:
+    devices = {t.device for t in tensors}
+    if len(devices) != 1:
+        raise ValueError(f"all tensors must be on one device, got {sorted(map(str, devices))}")
+    device = devices.pop()
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not {device}")
+    return device
+
+
+class _on_device:
+    """Makes a device the current one where it is not (launches go to the
+    current device's context)."""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+def _norm_partials(lib, entries: np.ndarray, buffer: torch.Tensor, stream: int) -> int:
+    count = ctypes.c_int64(0)
+    _lib.check(lib.gs_grad_norm_partials(entries.ctypes.data, len(entries), buffer.data_ptr(), buffer.numel(),
+                                         ctypes.byref(count), stream), "gradient norm")
+    return count.value
+
+
+class FusedAdamW:
+    """AdamW over the tensors of ``params`` (name -> tensor, updated in place).
+
+    ``lr``: a float, or a one-element float32 tensor on the parameters' device
+    that each step reads there.  ``lr_scales`` / ``decay_scales``: per-name
+    factors of ``lr`` and ``weight_decay`` (1 where a name is missing).
+    ``state_bits``: 32 or 8.  ``master_weights``: keep float32 copies of the
+    16-bit parameters and round the parameters from them (call
+    ``sync_master`` after changing such parameters elsewhere).  ``max_norm``:
+    clip the gradients to this global norm inside the step.
+    ``skip_nonfinite``: leave parameters, moments and the step count as they
+    are when a gradient is not finite (a step with ``max_norm`` always does).
+
+    Parameters may be strided rows (a pool's columns); they may not overlap.
+    The optimizer belongs to one stream at a time, as its parameters do."""
+
+    def __init__(self, params: Dict[str, torch.Tensor], lr: Union[float, torch.Tensor] = 1e-3,
+                 betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 lr_scales: Optional[Dict[str, float]] = None, decay_scales: Optional[Dict[str, float]] = None,
+                 state_bits: int = 32, master_weights: bool = False, max_norm: Optional[float] = None,
+                 skip_nonfinite: bool = False):
+        if not params:
+            raise ValueError("no parameters")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"betas must be in [0, 1): {betas}")
+        if not (math.isfinite(eps) and float(np.float32(eps)) > 0.0):
+            raise ValueError(f"eps must be positive: {eps}")
+        if not (math.isfinite(weight_decay) and weight_decay >= 0.0):
+            raise ValueError(f"weight_decay must not be negative: {weight_decay}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32: {state_bits}")
+        for what, scales in (("lr_scales", lr_scales), ("decay_scales", decay_scales)):
+            unknown = set(scales or ()) - set(params)
+            if unknown:
+                raise ValueError(f"{what}: no parameter named {sorted(unknown)}")
+            if not all(math.isfinite(x) for x in (scales or {}).values()):
+                raise ValueError(f"{what} must be finite")
+        self.names = list(params)
+        self._params = [params[k] for k in self.names]
+        self._rows = []
+        for name, p in params.items():
+            _check_tensor(f"parameter {name!r}", p)
+            rows = rows_of(p)
+            if rows is None:
+                raise ValueError(f"parameter {name!r}: strides {tuple(p.stride())} of shape {tuple(p.shape)} are "
+                                 "neither dense nor rows at one distance")
+            self._rows.append(rows)
+        both = overlapping(self._params, self._rows)
+        if both is not None:
+            raise ValueError(f"parameters {self.names[both[0]]!r} and {self.names[both[1]]!r} share memory")
+        self.device = _check_cuda(self._params)
+        self.beta1, self.beta2 = float(betas[0]), float(betas[1])
+        self.eps = float(eps)
+        self.weight_decay = float(weight_decay)
+        self.state_bits = state_bits
+        self.skip_nonfinite = bool(skip_nonfinite)
+        self.lr = lr
+        self.max_norm = max_norm
+        self._lr_value()
+        self._norm_limit()
+        # aliases keep the memory that the entries point to alive whatever happens to the caller's tensors
+        self._aliases = [p.detach() for p in self._params]
+        self._ptrs = list(map(_data_ptr, self._params))
+        self._shapes = list(map(_shape, self._params))
+        n = len(self._params)
+        sizes = [p.numel() for p in self._params]
+        room = [-(-s // BLOCK) * BLOCK for s in sizes]
+        self.offsets = {k: o for k, o in zip(self.names, np.cumsum([0] + room[:-1]).tolist())}
+        self.slab_elements = sum(room)
+        e = np.zeros(n, _ENTRY)
+        e["param"], e["n"] = self._ptrs, sizes
+        e["state"] = [self.offsets[k] for k in self.names]
+        e["cols"] = [c for c, _ in self._rows]
+        e["param_stride"] = [s for _, s in self._rows]
+        e["param_type"] = [TYPES[p.dtype] for p in self._params]
+        e["lr_scale"] = [float((lr_scales or {}).get(k, 1.0)) for k in self.names]
+        e["decay"] = [self.weight_decay * float((decay_scales or {}).get(k, 1.0)) for k in self.names]
+        self._entries = e
+        dt = torch.float32 if state_bits == 32 else torch.uint8
+        self.m = torch.zeros(self.slab_elements, dtype=dt, device=self.device)
+        self.v = torch.zeros(self.slab_elements, dtype=dt, device=self.device)
+        blocks = self.slab_elements // BLOCK if state_bits == 8 else 0
+        self.m_exp = torch.zeros(blocks, dtype=torch.uint8, device=self.device)
+        self.v_exp = torch.zeros(blocks, dtype=torch.uint8, device=self.device)
+        self._control = torch.zeros(2, dtype=torch.int64, device=self.device)
+        self.master_slab: Optional[torch.Tensor] = None
+        if master_weights and any(p.dtype != torch.float32 for p in self._params):
+            self.master_slab = torch.zeros(self.slab_elements, dtype=torch.float32, device=self.device)
+            self.sync_master()
+        self._state = _lib.GsAdamWState(_lib.ptr(self.m), _lib.ptr(self.v), _lib.ptr(self.m_exp),
+                                        _lib.ptr(self.v_exp), _lib.ptr(self.master_slab), _lib.ptr(self._control),
+                                        state_bits)
+        self._partials: Optional[torch.Tensor] = None
+        if max_norm is not None or skip_nonfinite:
+            self._partials_buffer(_lib.lib())
+
+    # ------------------------------------------------------------------ checks
+    def _lr_value(self) -> Tuple[float, Optional[int]]:
+        lr = self.lr
+        if isinstance(lr, torch.Tensor):
+            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != self.device:
+                raise ValueError("a tensor lr is one float32 on the parameters' device")
+            return 0.0, lr.data_ptr()
+        lr = float(lr)
+        if not (math.isfinite(lr) and lr >= 0.0):
+            raise ValueError(f"lr must not be negative: {lr}")
+        return lr, None
+
+    def _norm_limit(self) -> float:
+        if self.max_norm is None:
+            return math.inf
+        limit = float(self.max_norm)
+        if not limit > 0.0:
+            raise ValueError(f"max_norm must be positive: {self.max_norm}")
+        return limit
+
+    def _partials_buffer(self, lib) -> torch.Tensor:
+        if self._partials is None:
+            with _on_device(self.device):
+                size = lib.gs_grad_norm_max_partials(len(self._params))
+            self._partials = torch.empty(size, dtype=torch.float64, device=self.device)
+        return self._partials
+
+    def _refresh(self) -> None:
+        """The parameters' memory was replaced (``p.data = ...``): takes the new
+        memory when it has the old form."""
+        for k, (name, p) in enumerate(zip(self.names, self._params)):
+            if p.data_ptr() == self._ptrs[k]:
+                continue
+            if p.dtype != self._aliases[k].dtype or p.shape != self._shapes[k] or p.device != self.device or \
+                    rows_of(p) != self._rows[k]:
+                raise ValueError(f"parameter {name!r} no longer has the type, shape, strides or device it was "
+                                 "given with")
+        both = overlapping(self._params, self._rows)
+        if both is not None:
+            raise ValueError(f"parameters {self.names[both[0]]!r} and {self.names[both[1]]!r} share memory")
+        self._aliases = [p.detach() for p in self._params]
+        self._ptrs = list(map(_data_ptr, self._params))
+        self._entries["param"] = self._ptrs
+
+    def _with_grads(self, entries: np.ndarray, names: Sequence[str], shapes: Sequence[torch.Size],
+                    grads: List[torch.Tensor], what: str = "gradient") -> List[torch.Tensor]:
+        """Fills the entries' second tensor from ``grads`` (checked against
+        ``shapes``); returns the tensors that must outlive the launch."""
+        if not all(isinstance(g, torch.Tensor) for g in grads) or \
+                any(g.layout != torch.strided or g.dtype not in TYPES for g in grads):
+            for name, g in zip(names, grads):
+                _check_tensor(f"{what} of {name!r}", g)
+        if list(map(_shape, grads)) != list(shapes):
+            for name, s, g in zip(names, shapes, grads):
+                if g.shape != s:
+                    raise ValueError(f"{what} of {name!r} has shape {tuple(g.shape)}, not {tuple(s)}")
+        if set(map(_device_index, grads)) != {self.device.index}:
+            raise ValueError(f"every {what} must be on {self.device}")
+        entries["grad_type"] = [TYPES[d] for d in map(_dtype, grads)]
+        entries["grad_stride"] = entries["cols"]
+        if not all(map(_is_contiguous, grads)):
+            grads = list(grads)
+            for k, g in enumerate(grads):
+                if g.is_contiguous():
+                    continue
+                rows = rows_of(g)
+                cols, stride = int(entries["cols"][k]), int(entries["param_stride"][k])
+                if rows is not None and rows[0] == cols:
+                    entries["grad_stride"][k] = rows[1]
+                elif rows is not None and cols == stride:  # a dense parameter takes the gradient's rows
+                    entries["cols"][k] = entries["param_stride"][k] = rows[0]
+                    entries["grad_stride"][k] = rows[1]
+                else:
+                    grads[k] = g.contiguous()
+        entries["grad"] = list(map(_data_ptr, grads))
+        return grads
+
+    # ------------------------------------------------------------------ the step
+    def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_scale: float = 1.0) -> Optional[torch.Tensor]:
+        """One step on the current stream.  ``grads``: name -> gradient (default:
+        the parameters' ``.grad``); a parameter without one keeps its values and
+        moments, and a step without any does nothing.  ``grad_scale`` multiplies
+        every gradient first (the inverse of a loss scale).  Returns the global
+        norm of the scaled gradients before clipping as a device scalar when
+        ``max_norm`` or ``skip_nonfinite`` asks for it, else None."""
+        lib = _lib.lib()
+        if grads is None:
+            found = [p.grad for p in self._params]
+        else:
+            if not grads.keys() <= self.offsets.keys():
+                raise ValueError(f"no parameter named {sorted(set(grads) - set(self.names))}")
+            found = list(map(grads.get, self.names))
+        if not math.isfinite(grad_scale):
+            raise ValueError(f"grad_scale must be finite: {grad_scale}")
+        lr, lr_device = self._lr_value()
+        limit = self._norm_limit()
+        if list(map(_data_ptr, self._params)) != self._ptrs:
+            self._refresh()
+        names, shapes, params = self.names, self._shapes, self._params
+        if any(g is None for g in found):
+            on = [k for k, g in enumerate(found) if g is not None]
+            entries = self._entries[on]
+            names, shapes, params, found = ([x[k] for k in on] for x in (names, shapes, params, found))
+        else:
+            entries = self._entries.copy()
+        with_norm = self.max_norm is not None or self.skip_nonfinite
+        norm = None
+        with _on_device(self.device):
+            if with_norm:
+                norm = torch.empty((), dtype=torch.float32, device=self.device)
+            if not params or not int(entries["n"].sum()):
+                return norm.zero_() if with_norm else None
+            keep = self._with_grads(entries, names, shapes, found)
+            stream = _lib.stream_ptr(self.device)
+            s = _lib.GsAdamWSettings(lr, self.beta1, self.beta2, self.eps, grad_scale, lr_device, None, 0, limit, None)
+            if with_norm:
+                buffer = self._partials_buffer(lib)
+                s.num_partials = _norm_partials(lib, entries, buffer, stream)
+                s.norm_partials = buffer.data_ptr()
+                s.norm_out = norm.data_ptr()
+            _lib.check(lib.gs_adamw_step(entries.ctypes.data, len(entries), self._state, s, stream), "adamw step")
+            del keep
+        torch.autograd.graph.increment_version(params)
+        return norm
+
+    # ------------------------------------------------------------------ state
+    @property
+    def t(self) -> int:
+        """Steps taken (read from the device: a host sync)."""
+        return int(self._control[0])
+
+    @t.setter
+    def t(self, value: int) -> None:
+        if value < 0:
+            raise ValueError(f"the step count must not be negative: {value}")
+        self._control[0] = int(value)
+
+    def _views(self, slab: torch.Tensor) -> Dict[str, torch.Tensor]:
+        return {k: slab[self.offsets[k]:self.offsets[k] + s.numel()].view(s)
+                for k, s in zip(self.names, self._shapes)}
+
+    def moment_slabs(self, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """m and v as flat slabs (``offsets`` gives each tensor's place; the
+        padding between them is zero).  The optimizer's own buffers when the
+        moments are float32 and ``dtype`` is too, else new tensors; bfloat16
+        holds every value of the 8-bit form exactly."""
+        if self.state_bits == 32:
+            return self.m.to(dtype), self.v.to(dtype)
+        return _dequantize(self.m, self.v, self.m_exp, self.v_exp, dtype)
+
+    def moments(self, dtype: torch.dtype = torch.float32) -> Tuple[Dict[str, torch.Tensor], Dict[str, torch.Tensor]]:
+        """``moment_slabs`` as name -> tensor of the parameter's shape."""
+        m, v = self.moment_slabs(dtype)
+        return self._views(m), self._views(v)
+
+    def load_moments(self, m: Dict[str, torch.Tensor], v: Dict[str, torch.Tensor], t: Optional[int] = None) -> None:
+        """Sets every parameter's moments (tensors of the parameters' shapes on
+        their device, any of the three types; v must not be negative) and the
+        step count.  With 8-bit moments values that the form holds are kept
+        exactly and others are rounded with the step count's offsets."""
+        if set(m) != set(self.names) or set(v) != set(self.names):
+            raise ValueError("moments for exactly the optimizer's parameters are needed")
+        ml, vl = [m[k] for k in self.names], [v[k] for k in self.names]
+        for what, tensors in (("moment m", ml), ("moment v", vl)):
+            for name, x in zip(self.names, tensors):
+                _check_tensor(f"{what} of {name!r}", x)
+        if t is not None:
+            if t < 0:
+                raise ValueError(f"the step count must not be negative: {t}")
+        with _on_device(self.device):
+            entries = np.zeros(len(ml), _ENTRY)
+            entries["n"], entries["state"] = self._entries["n"], self._entries["state"]
+            entries["cols"] = entries["param_stride"] = np.maximum(entries["n"], 1)
+            keep = self._with_grads(entries, self.names, self._shapes, [x.contiguous() for x in ml], "moment m")
+            for a, b in (("param", "grad"), ("param_type", "grad_type")):
+                entries[a] = entries[b]
+            keep = keep + self._with_grads(entries, self.names, self._shapes, [x.contiguous() for x in vl], "moment v")
+            if t is None:
+                t = self.t if self.state_bits == 8 else None
+            else:
+                self._control[0].fill_(int(t))
+            if self.state_bits == 32:
+                for slab, src in ((self.m, ml), (self.v, vl)):
+                    for dst, x in zip(self._views(slab).values(), src):
+                        dst.copy_(x)
+                return
+            lib = _lib.lib()
+            _lib.check(lib.gs_moments8_quantize(entries.ctypes.data, len(entries), self.m.data_ptr(),
+                                                self.v.data_ptr(), self.m_exp.data_ptr(), self.v_exp.data_ptr(),
+                                                int(t), _lib.stream_ptr(self.device)), "8-bit moments")
+            del keep
+
+    def sync_master(self) -> None:
+        """Takes the float32 master copies from the parameters again."""
+        if self.master_slab is not None:
+            for dst, p in zip(self._views(self.master_slab).values(), self._params):
+                dst.copy_(p.detach())
+
+    def state_dict(self) -> Dict[str, object]:
+        """A copy of the state: the moments in the form they are held in, the
+        master copies, the step count and the layout."""
+        d = {"state_bits": self.state_bits, "t": self.t, "shapes": {k: tuple(s) for k, s in zip(self.names, self._shapes)},
+             "m": self.m.clone(), "v": self.v.clone(), "m_exp": self.m_exp.clone(), "v_exp": self.v_exp.clone()}
+        if self.master_slab is not None:
+            d["master"] = self.master_slab.clone()
+        return d
+
+    def load_state_dict(self, d: Dict[str, object]) -> None:
+        """Restores a ``state_dict`` of the same parameters (names in the same
+        order, and shapes); moments held in the other number of bits are
+        converted."""
+        if list(d["shapes"].items()) != [(k, tuple(s)) for k, s in zip(self.names, self._shapes)]:
+            raise ValueError("the state belongs to other parameters")
+        bits = d["state_bits"]
+        m, v = d["m"].to(self.device), d["v"].to(self.device)
+        if self.master_slab is not None:
+            if "master" in d:
+                self.master_slab.copy_(d["master"])
+            else:
+                self.sync_master()
+        if bits == self.state_bits:
+            for dst, src in ((self.m, m), (self.v, v), (self.m_exp, d["m_exp"]), (self.v_exp, d["v_exp"])):
+                dst.copy_(src)
+            self.t = d["t"]
+            return
+        if bits == 8:
+            m, v = _dequantize(m, v, d["m_exp"].to(self.device), d["v_exp"].to(self.device), torch.float32)
+        self.load_moments(self._views(m), self._views(v), t=d["t"])
+
+
+def _dequantize(m, v, m_exp, v_exp, dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"8-bit moments are read as float32 or bfloat16, not {dtype}")
+    lib = _lib.lib()
+    with _on_device(m.device):
+        mo = torch.empty(m.numel(), dtype=dtype, device=m.device)
+        vo = torch.empty(v.numel(), dtype=dtype, device=v.device)
+        _lib.check(lib.gs_moments8_dequantize(m.data_ptr(), v.data_ptr(), m_exp.data_ptr(), v_exp.data_ptr(),
+                                              m.numel(), TYPES[dtype], mo.data_ptr(), vo.data_ptr(),
+                                              _lib.stream_ptr(m.device)), "moment values")
+    return mo, vo
+
+
+Tensors = Union[Dict[str, torch.Tensor], Sequence[torch.Tensor]]
+
+
+def _named(tensors: Tensors) -> Dict:
+    return dict(tensors) if isinstance(tensors, dict) else dict(enumerate(tensors))
+
+
+def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = None) -> torch.Tensor:
+    """Scales the gradients (name -> tensor, or a sequence) by ``max_norm`` over
+    their global norm where that exceeds ``max_norm``, in place, or into the
+    tensors of ``out`` (same names and shapes, any of the three types; written
+    in any case).  Returns the norm before as a device scalar; where it is not
+    finite nothing is scaled.  Strided rows are taken as they are; written
+    tensors may not overlap one another or other gradients."""
+    max_norm = float(max_norm)
+    if not max_norm > 0.0:
+        raise ValueError(f"max_norm must be positive: {max_norm}")
+    src = _named(grads)
+    dst = src if out is None else _named(out)
+    if not src:
+        raise ValueError("no gradients")
+    if src.keys() != dst.keys():
+        raise ValueError("out must have the gradients' names")
+    gl, ol = list(src.values()), [dst[k] for k in src]
+    entries = np.zeros(len(gl), _ENTRY)
+    for k, (name, g, o) in enumerate(zip(src, gl, ol)):
+        _check_tensor(f"gradient {name!r}", g)
+        if o is not g:
+            _check_tensor(f"out {name!r}", o)
+            if o.shape != g.shape:
+                raise ValueError(f"out {name!r} has shape {tuple(o.shape)}, not {tuple(g.shape)}")
+    g_rows = list(map(rows_of, gl))
+    o_rows = g_rows if out is None else list(map(rows_of, ol))
+    for k, name in enumerate(src):
+        if o_rows[k] is None:
+            raise ValueError(f"{'gradient' if out is None else 'out'} {name!r}: strides {tuple(ol[k].stride())} of "
+                             f"shape {tuple(ol[k].shape)} are neither dense nor rows at one distance")
+    both = overlapping(ol, o_rows)
+    if both is not None:
+        raise ValueError("written tensors share memory")
+    if out is not None:
+        _check_apart(gl, g_rows, ol, o_rows)
+    device = _check_cuda(gl + ol)
+    lib = _lib.lib()
+    with _on_device(device):
+        for k in range(len(gl)):
+            dense = g_rows[k] is not None and g_rows[k][0] == g_rows[k][1]
+            if g_rows[k] is None or not (dense or o_rows[k][0] in (o_rows[k][1], g_rows[k][0])):
+                gl[k] = gl[k].contiguous()
+                g_rows[k] = rows_of(gl[k])
+                dense = True
+            cols = o_rows[k][0] if dense else g_rows[k][0]
+            entries[k] = (ol[k].data_ptr(), gl[k].data_ptr(), gl[k].numel(), 0, cols,
+                          cols if o_rows[k][0] == o_rows[k][1] else o_rows[k][1], cols if dense else g_rows[k][1],
+                          TYPES[ol[k].dtype], TYPES[gl[k].dtype], 1.0, 0.0)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        if not int(entries["n"].sum()):
+            return norm.zero_()
+        stream = _lib.stream_ptr(device)
+        partials = torch.empty(lib.gs_grad_norm_max_partials(len(entries)), dtype=torch.float64, device=device)
+        count = _norm_partials(lib, entries, partials, stream)
+        _lib.check(lib.gs_clip_gradients(entries.ctypes.data, len(entries), partials.data_ptr(), count, max_norm,
+                                         norm.data_ptr(), stream), "clip gradients")
+    torch.autograd.graph.increment_version(ol)
+    return norm
+
+
+def _check_apart(gl, g_rows, ol, o_rows) -> None:
+    """A written tensor may be its own gradient's memory, but no other's."""
+    spans = sorted(_span(o, r) for o, r in zip(ol, o_rows) if o.numel())
+    starts, ends = [s for s, _ in spans], [e for _, e in spans]
+    if not spans:
+        return
+    for k, g in enumerate(gl):
+        if not g.numel() or (g.data_ptr() == ol[k].data_ptr() and g.dtype == ol[k].dtype and
+                             g.stride() == ol[k].stride()):
+            continue
+        lo = g.data_ptr()
+        hi = lo + (sum((d - 1) * s for d, s in zip(g.shape, g.stride())) + 1) * g.element_size()
+        at = int(np.searchsorted(starts, hi)) - 1
+        # spans of strided outputs may nest, so every span that starts before ``hi`` counts
+        if at >= 0 and max(ends[:at + 1]) > lo:
+            raise ValueError("a written tensor shares memory with another gradient")

@@ -1,0 +1,166 @@
+// The global norm of many gradients and their clipping by it.
+//
+//   norm = |grad_scale| sqrt(sum over all tensors of g^2)
+//   g'   = g * max_norm / norm   when norm > max_norm
+//
+// The squares are formed and summed in 64 bits: a norm over tens of millions of
+// elements is then correct to float32's last bit whatever the order, is finite in
+// float32 wherever it lies in float32's range, and the order is fixed (each block writes one
+// partial sum, every consumer adds them in index order), so a run repeats bit for
+// bit.  Finding the norm has to read every gradient before the first may be
+// scaled; only gradients that still lie in the 126 MB L2 are not read from
+// memory twice.
+#include <math.h>
+
+#include "multi_tensor.cuh"
+
+namespace gs {
+
+constexpr int kNormBlocksPerSm = 4;
+
+__device__ __forceinline__ double sum_squares8(const float (&x)[8]) {
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s = fma((double)x[k], (double)x[k], s);
+    return s;
+}
+
+template <int kCap>
+__global__ void __launch_bounds__(kMultiThreads) grad_norm_kernel(const __grid_constant__ TensorTable<kCap> tab,
+                                                                  double* partials) {
+    pdl_wait();
+    int c, end;
+    block_share(tab, c, end);
+    double sum = 0.0;
+    if (c < end) {
+        int ti = find_tensor(tab, c);
+        for (; c < end; ++c) {
+            while (c >= tab.first[ti + 1]) ++ti;
+            const TensorEntry& e = tab.e[ti];
+            const int64_t i = (int64_t)(c - tab.first[ti]) * kChunk + threadIdx.x * kPerThread;
+            if (i >= e.n) continue;
+            float g[8];
+            if (e.grad_vec && i + kPerThread <= e.n)
+                unpack8(load_raw8(e.grad, i, e.grad_type), e.grad_type, g);
+            else
+                load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, g);
+            sum += sum_squares8(g);
+        }
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+}
+
+template <int kCap>
+__global__ void __launch_bounds__(kMultiThreads) grad_clip_kernel(const __grid_constant__ TensorTable<kCap> tab,
+                                                                  const double* partials, int64_t num_partials,
+                                                                  double max_norm, float* norm_out) {
+    __shared__ float factor;
+    pdl_wait();
+    const double sq = sum_partials(partials, num_partials);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(sq);
+        // a norm that is not finite in float32 leaves the gradients as they are
+        factor = norm > max_norm && isfinite((float)norm) ? (float)(max_norm / norm) : 1.0f;
+        if (blockIdx.x == 0 && norm_out) *norm_out = (float)norm;
+    }
+    __syncthreads();
+    const float f = factor;
+    int c, end;
+    block_share(tab, c, end);
+    if (c >= end) return;
+    int ti = find_tensor(tab, c);
+    for (; c < end; ++c) {
+        while (c >= tab.first[ti + 1]) ++ti;
+        const TensorEntry& e = tab.e[ti];
+        if (f == 1.0f && e.param == e.grad) continue;  // in place and not clipped
+        const int64_t i = (int64_t)(c - tab.first[ti]) * kChunk + threadIdx.x * kPerThread;
+        if (i >= e.n) continue;
+        const bool whole = i + kPerThread <= e.n;
+        float g[8];
+        if (e.grad_vec && whole)
+            unpack8(load_raw8(e.grad, i, e.grad_type), e.grad_type, g);
+        else
+            load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g[k] = __fmul_rn(g[k], f);
+        if (e.param_vec && whole)
+            store_vec8(e.param, i, e.param_type, g);
+        else
+            store_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, g);
+    }
+}
+
+template <int kCap>
+static int norm_launches(const gs_tensor* t, int64_t count, double* partials, int64_t capacity, int64_t* written,
+                         bool launch, cudaStream_t stream) {
+    TensorTable<kCap> tab;
+    int64_t left = live_tensors(t, count), done = 0;
+    for (int64_t at = 0; left > 0;) {
+        at = fill_table(tab, t, at, count);
+        left -= tab.count;
+        const int grid = table_grid(tab, kNormBlocksPerSm);
+        if (launch) {
+            if (done + grid > capacity)
+                return set_error(GS_ERR_CAPACITY, "grad_norm: %lld partial sums do not fit", (long long)capacity);
+            double* out = partials + done;
+            void* args[] = {&tab, &out};
+            GS_TRY(launch_table("grad_norm_kernel", (const void*)grad_norm_kernel<kCap>, grid, stream, args));
+        }
+        done += grid;
+    }
+    *written = done;
+    return GS_OK;
+}
+
+template <int kCap>
+static int clip_launches(const gs_tensor* t, int64_t count, const double* partials, int64_t num_partials,
+                         double max_norm, float* norm_out, cudaStream_t stream) {
+    TensorTable<kCap> tab;
+    int64_t left = live_tensors(t, count);
+    for (int64_t at = 0; left > 0;) {
+        at = fill_table(tab, t, at, count);
+        left -= tab.count;
+        void* args[] = {&tab, &partials, &num_partials, &max_norm, &norm_out};
+        GS_TRY(launch_table("grad_clip_kernel", (const void*)grad_clip_kernel<kCap>,
+                            table_grid(tab, kNormBlocksPerSm), stream, args));
+    }
+    return GS_OK;
+}
+
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int64_t gs_grad_norm_max_partials(int64_t count) {
+    // at most one wave of blocks for every table of tensors
+    if (count <= 0) return 0;
+    const int64_t cap = count <= kSmallTable ? kSmallTable : kLargeTable;
+    return (count + cap - 1) / cap * (int64_t)sm_count() * kNormBlocksPerSm;
+}
+
+extern "C" int gs_grad_norm_partials(const gs_tensor* tensors, int64_t count, double* partials, int64_t capacity,
+                                     int64_t* num_partials, gs_stream_t stream) {
+    GS_REQUIRE(num_partials, "grad_norm: null count");
+    *num_partials = 0;
+    GS_TRY(check_tensors("grad_norm", tensors, count, kNeedGrad));
+    if (live_tensors(tensors, count) == 0) return GS_OK;
+    GS_REQUIRE(partials && capacity > 0, "grad_norm: null partial sums");
+    const cudaStream_t st = (cudaStream_t)stream;
+    return count <= kSmallTable
+               ? norm_launches<kSmallTable>(tensors, count, partials, capacity, num_partials, true, st)
+               : norm_launches<kLargeTable>(tensors, count, partials, capacity, num_partials, true, st);
+}
+
+extern "C" int gs_clip_gradients(const gs_tensor* tensors, int64_t count, const double* partials,
+                                 int64_t num_partials, double max_norm, float* norm_out, gs_stream_t stream) {
+    GS_REQUIRE(max_norm > 0.0, "clip_gradients: max_norm must be positive");
+    GS_REQUIRE(num_partials >= 0, "clip_gradients: bad partial count");
+    GS_TRY(check_tensors("clip_gradients", tensors, count, kNeedParam | kNeedGrad));
+    if (live_tensors(tensors, count) == 0) return GS_OK;
+    GS_REQUIRE(partials, "clip_gradients: null partial sums");
+    const cudaStream_t st = (cudaStream_t)stream;
+    return count <= kSmallTable
+               ? clip_launches<kSmallTable>(tensors, count, partials, num_partials, max_norm, norm_out, st)
+               : clip_launches<kLargeTable>(tensors, count, partials, num_partials, max_norm, norm_out, st);
+}

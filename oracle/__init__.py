@@ -15,6 +15,8 @@ Modules and the reference code each one follows:
 * ``oracle.adam`` — the fused Metal Adam (``src/mlx_extensions.cpp:102-152``,
   restated in C in ``oracle/adam_a1.c``) and the pure-MLX Adam
   (``mlx_gsplat/optimizer.py:146-175``).
+* ``oracle.adamw`` — AdamW over separate tensors and the 8-bit form of its
+  moments (no reference counterpart).
 * ``oracle.allocator`` — ``PointerStableChunkedAllocator``
   (``mlx_gsplat/allocator.py:8-292``), including its LIFO free-list order.
 * ``oracle.densify`` — the trainer's densify/prune policy and child values

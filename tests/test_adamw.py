@@ -1,0 +1,230 @@
+"""``FusedAdamW`` / ``clip_gradients`` on the CPU: refusals, the layout rules,
+the C ABI's argument checks, and the 8-bit form's properties (in the oracle)."""
+import ctypes
+import math
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_gsplat_b200 import FusedAdamW, _lib, clip_gradients
+from mlx_gsplat_b200.adamw import _ENTRY, overlapping, rows_of
+from oracle import adamw as oadamw
+
+built = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
+
+
+# ---------------------------------------------------------------- layouts
+def test_rows_of():
+    slab = torch.zeros(10, 60)
+    assert rows_of(slab) == (600, 600)
+    assert rows_of(slab[:, 4:7]) == (3, 60)
+    assert rows_of(slab[:, 7:8]) == (1, 60)
+    assert rows_of(slab[3:7]) == (240, 240)
+    assert rows_of(slab[::2]) == (60, 120)
+    assert rows_of(torch.zeros(4, 5, 6)[:, :, :3]) == (3, 6)
+    assert rows_of(torch.zeros(4, 5, 6)[:, :2]) == (12, 30)
+    assert rows_of(torch.zeros(4, 5, 6)[:, :2, :3]) is None  # two strides
+    assert rows_of(slab.t()) is None
+    assert rows_of(torch.zeros(3, 1).expand(3, 4)) is None
+    assert rows_of(torch.zeros(())) == (1, 1)
+    assert rows_of(torch.zeros(0, 4)) == (1, 1)
+
+
+def _over(*tensors):
+    return overlapping(tensors, [rows_of(t) for t in tensors])
+
+
+def test_overlap():
+    slab = torch.zeros(10, 60)
+    assert _over(slab[:, 0:4], slab[:, 4:7], slab[:, 7:8], slab[:, 8:60]) is None
+    assert _over(slab[:, 0:5], slab[:, 4:7]) is not None
+    assert _over(slab, slab) is not None
+    assert _over(slab, slab[:, 3:5]) is not None
+    assert _over(slab[:5], slab[5:]) is None
+    assert _over(slab[:5, :3], slab[5:, :3], slab[4:6, 4:5]) is None
+    flat = torch.zeros(100)
+    assert _over(flat[:50], flat[50:]) is None
+    assert _over(flat[:51], flat[50:]) is not None
+    assert _over(flat, torch.zeros(100), flat[0:0]) is None
+    # one pitch, columns that wrap past the row's end
+    assert _over(flat[:90].view(9, 10)[:, 8:], flat[9:99].view(9, 10)[:, 0:2]) is not None
+    # pitches of which one divides the other; pitches without a common distance
+    assert _over(flat.view(10, 10)[:, :2], flat[2:82].view(4, 20)[:, :2]) is None
+    assert _over(flat.view(10, 10)[:, :2], flat[11:91].view(4, 20)[:, :2]) is not None
+    assert _over(flat.view(10, 10)[:, :2], flat[2:79].view(7, 11)[:, :2]) is not None
+
+
+# ---------------------------------------------------------------- refusals
+@pytest.mark.parametrize("kw,msg", [
+    (dict(betas=(1.0, 0.9)), "betas"), (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=0.0), "eps"),
+    (dict(eps=1e-60), "eps"), (dict(eps=math.nan), "eps"), (dict(weight_decay=-1.0), "weight_decay"),
+    (dict(state_bits=16), "state_bits"), (dict(lr_scales={"b": 1.0}), "lr_scales"),
+    (dict(decay_scales={"a": math.inf}), "decay_scales"),
+])
+def test_bad_settings(kw, msg):
+    with pytest.raises(ValueError, match=msg):
+        FusedAdamW({"a": torch.zeros(3)}, **kw)
+
+
+@pytest.mark.parametrize("params,msg", [
+    ({}, "no parameters"),
+    ({"a": torch.zeros(3, dtype=torch.float64)}, "float64"),
+    ({"a": torch.zeros(3, dtype=torch.int32)}, "int32"),
+    ({"a": torch.zeros(3, 4).t()}, "strides"),
+    ({"a": torch.zeros(3).to_sparse()}, "sparse"),
+    ({"a": torch.zeros(1).expand(4)}, "strides"),
+    ({"a": torch.zeros(3)}, "CUDA"),
+])
+def test_bad_parameters(params, msg):
+    with pytest.raises(ValueError, match=msg):
+        FusedAdamW(params)
+
+
+def test_shared_parameters():
+    x = torch.zeros(8)
+    with pytest.raises(ValueError, match="share memory"):
+        FusedAdamW({"a": x, "b": x})
+    with pytest.raises(ValueError, match="share memory"):
+        FusedAdamW({"a": x[:5], "b": x[4:]})
+    with pytest.raises(TypeError):
+        FusedAdamW({"a": [1.0]})
+
+
+def test_bad_clipping():
+    g = torch.zeros(8)
+    for bad in (0.0, -1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            clip_gradients([g], bad)
+    with pytest.raises(ValueError, match="no gradients"):
+        clip_gradients({}, 1.0)
+    with pytest.raises(ValueError, match="CUDA"):
+        clip_gradients([g], 1.0)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_gradients([g, g], 1.0)
+    with pytest.raises(ValueError, match="names"):
+        clip_gradients({"a": g}, 1.0, out={"b": g})
+    with pytest.raises(ValueError, match="shape"):
+        clip_gradients({"a": g}, 1.0, out={"a": torch.zeros(7)})
+    with pytest.raises(ValueError, match="strides"):
+        clip_gradients([torch.zeros(3, 4).t()], 1.0)
+    big = torch.zeros(16)
+    with pytest.raises(ValueError, match="another gradient"):
+        clip_gradients([big[:8]], 1.0, out=[big[4:12]])
+    with pytest.raises(ValueError, match="another gradient"):
+        clip_gradients([big[:8], big[8:]], 1.0, out=[big[8:], torch.zeros(8)])
+    with pytest.raises(ValueError, match="CUDA"):  # its own gradient's memory is fine
+        clip_gradients([big[:8]], 1.0, out=[big[:8]])
+
+
+# ---------------------------------------------------------------- C ABI checks (no CUDA call is reached)
+def _entry(**kw):
+    e = np.zeros(1, _ENTRY)
+    e["param"], e["grad"], e["n"], e["cols"] = 4096, 8192, 5, 5
+    e["param_stride"] = e["grad_stride"] = 5
+    for k, v in kw.items():
+        e[k] = v
+    return e
+
+
+def _state(bits=32, **kw):
+    d = dict(m=1 << 20, v=2 << 20, m_exp=3 << 20, v_exp=4 << 20, master=None, control=5 << 20)
+    d.update(kw)
+    return _lib.GsAdamWState(d["m"], d["v"], d["m_exp"], d["v_exp"], d["master"], d["control"], bits)
+
+
+def _settings(**kw):
+    d = dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, lr_device=None, norm_partials=None,
+             num_partials=0, max_norm=math.inf, norm_out=None)
+    d.update(kw)
+    return _lib.GsAdamWSettings(*d.values())
+
+
+@built
+@pytest.mark.parametrize("entry,state,settings,msg", [
+    (dict(n=-1), {}, {}, b"element count"), (dict(cols=0), {}, {}, b"row length"), (dict(state=100), {}, {}, b"256"),
+    (dict(param=0), {}, {}, b"null param"), (dict(grad=0), {}, {}, b"null grad"),
+    (dict(param_type=3), {}, {}, b"type"), (dict(grad_type=-1), {}, {}, b"type"), (dict(grad=8194), {}, {}, b"misaligned"),
+    (dict(param_stride=4), {}, {}, b"stride"), ({}, dict(bits=16), {}, b"32 or 8"), ({}, dict(m=None), {}, b"null"),
+    ({}, dict(control=None), {}, b"null"), ({}, dict(bits=8, m_exp=None), {}, b"exponents"),
+    ({}, dict(v=(2 << 20) + 4), {}, b"aligned"), ({}, {}, dict(beta1=1.0), b"betas"), ({}, {}, dict(eps=0.0), b"eps"),
+    ({}, {}, dict(grad_scale=math.nan), b"grad_scale"), ({}, {}, dict(lr=math.inf), b"lr"),
+    ({}, {}, dict(norm_partials=4096, num_partials=1, max_norm=0.0), b"max_norm"),
+])
+def test_step_refuses(entry, state, settings, msg):
+    lib = _lib.load()
+    e = _entry(**entry)
+    st = lib.gs_adamw_step(e.ctypes.data, 1, _state(**state), _settings(**settings), None)
+    assert st == _lib.GS_ERR_INVALID and msg in lib.gs_last_error(), lib.gs_last_error()
+
+
+@built
+def test_other_entries_refuse_and_skip_nothing_to_do():
+    lib = _lib.load()
+    assert _ENTRY.itemsize == 80 and ctypes.sizeof(_lib.GsAdamWState) == 56 and ctypes.sizeof(_lib.GsAdamWSettings) == 80
+    none = _entry(n=0)
+    got = ctypes.c_int64(7)
+    assert lib.gs_adamw_step(none.ctypes.data, 1, _state(), _settings(), None) == 0
+    assert lib.gs_adamw_step(None, 0, _state(), _settings(), None) == 0
+    assert lib.gs_adamw_step(None, 1, _state(), _settings(), None) == _lib.GS_ERR_INVALID
+    assert lib.gs_adamw_step(none.ctypes.data, 1, None, _settings(), None) == _lib.GS_ERR_INVALID
+    assert lib.gs_grad_norm_partials(none.ctypes.data, 1, None, 0, ctypes.byref(got), None) == 0 and got.value == 0
+    e = _entry()
+    assert lib.gs_grad_norm_partials(e.ctypes.data, 1, None, 0, ctypes.byref(got), None) == _lib.GS_ERR_INVALID
+    assert lib.gs_grad_norm_partials(e.ctypes.data, 1, 4096, 8, None, None) == _lib.GS_ERR_INVALID
+    assert lib.gs_clip_gradients(e.ctypes.data, 1, 4096, 1, 0.0, None, None) == _lib.GS_ERR_INVALID
+    assert lib.gs_clip_gradients(e.ctypes.data, 1, None, 1, 1.0, None, None) == _lib.GS_ERR_INVALID
+    assert lib.gs_moments8_quantize(e.ctypes.data, 1, None, 4096, 4096, 4096, 0, None) == _lib.GS_ERR_INVALID
+    assert lib.gs_moments8_dequantize(4096, 4096, 4096, 4096, 100, 0, 4096, 4096, None) == _lib.GS_ERR_INVALID
+    assert lib.gs_moments8_dequantize(4096, 4096, 4096, 4096, 256, 2, 4096, 4096, None) == _lib.GS_ERR_INVALID
+    assert lib.gs_moments8_dequantize(None, None, None, None, 0, 0, None, None, None) == 0
+
+
+# ---------------------------------------------------------------- the 8-bit form
+def test_every_code_is_kept():
+    """A block of values on the grid is coded back to itself at any step."""
+    for positive in (False, True):
+        codes = np.arange(256, dtype=np.uint8)
+        if not positive:
+            codes[128] = 0  # a signed zero is kept as a code, checked apart
+        for e in (64, 100, 127, 180, 254):
+            x = oadamw.values(codes, np.array([e], np.uint8), positive)
+            assert np.isfinite(x).all()
+            for t in (0, 1, 12345):
+                c, got = oadamw.quantize(x, t, positive)
+                assert got[0] == e
+                np.testing.assert_array_equal(c, codes)
+
+
+@pytest.mark.parametrize("positive", [False, True], ids=["m", "v"])
+def test_rounding_is_unbiased_over_steps(positive):
+    """The mean over N steps of the values a fixed x is rounded to lies within D
+    of x in steps of the grid, D = (3 + (1 / ln(golden) + 2 / ln 3) ln N) / N, the
+    discrepancy bound of multiples of sqrt(2) (partial quotients at most 2)."""
+    rng = np.random.default_rng(3)
+    x = np.exp(rng.normal(0, 2, 512)).astype(np.float32)
+    x[::256] = 1e3  # keeps the blocks' exponents
+    N = 1000
+    total = np.zeros(512)
+    for t in range(N):
+        total += oadamw.values(*oadamw.quantize(x, t, positive), positive)
+    d = (3 + (1 / np.log((1 + 5 ** 0.5) / 2) + 2 / np.log(3)) * np.log(N)) / N
+    step = np.exp2(np.frexp(x.astype(np.float64))[1] - 4.0)
+    err = np.abs(total / N - x)
+    # The blocks' top, 1000 = 15.6 steps of 64, is rounded to 960 or to 1024, so the exponent alternates between
+    # those of 2^9 and 2^10, and m's lowest whole binade between 2^-5 and 2^-4.  Above it an element's step does
+    # not depend on the exponent and the bound holds; below, the step alternates with the top's offset, and what
+    # holds is that each rounding is off by less than the coarser step, 2^-4 / 8.
+    whole = x >= (0.0 if positive else 2.0 ** -4)
+    assert (err <= (d + 2.0 ** -20) * step)[whole].all()
+    assert (err[~whole] < 2.0 ** -7).all()
+
+
+def test_positive_v_stays_positive():
+    x = np.full(256, 1e-30, np.float32)
+    x[0] = 1.0
+    x[5] = 0.0
+    for t in range(50):
+        c, _ = oadamw.quantize(x, t, True)
+        assert c[5] == 0 and (np.delete(c, 5) > 0).all()

@@ -1,0 +1,578 @@
+"""``FusedAdamW`` and ``clip_gradients`` on the GPU against the oracle: moments
+equal float32 arithmetic bit for bit, parameters within the derived bound of the
+step in 64 bits, 8-bit codes equal the form written from real arithmetic."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_gsplat_b200 import (FusedAdamW, FusedMLXAdam, PointerStableChunkedAllocator, clip_gradients,
+                             frustum_culling_mlx, rasterize_gaussians_mlx, synthetic)
+from mlx_gsplat_b200.adamw import BLOCK
+from oracle import adamw as oadamw
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+HALF_STEP = {F32: 0.0, BF16: 2.0 ** -8, F16: 2.0 ** -11}  # a rounding to nearest, relative
+TINY = {F32: 0.0, BF16: 2.0 ** -134, F16: 2.0 ** -25}     # and below the normal range
+SIZES = [1, 7, 8, 9, 255, 256, 257, 0, 2047, 2048, 2049, 5003]
+
+
+def tensors(seed, shapes, dtype, scale=1.0, sparse=0.0):
+    gen = torch.Generator().manual_seed(seed)
+    out = {}
+    for k, s in shapes.items():
+        x = torch.randn(s, generator=gen) * torch.exp(2 * torch.randn(s, generator=gen)) * scale
+        x = torch.where(torch.rand(s, generator=gen) < sparse, 0.0, x)
+        out[k] = x.to(dtype).to(DEV)
+    return out
+
+
+def flat(t):
+    return t.detach().float().reshape(-1).cpu().numpy()
+
+
+def finite(t):
+    x = flat(t)
+    return np.where(np.isfinite(x), x, np.nan)
+
+
+class Reference:
+    """The oracle's state of one optimizer; ``step`` checks the optimizer against it."""
+
+    def __init__(self, opt, params):
+        self.opt, self.params = opt, params
+        self.p = {k: flat(p) for k, p in params.items()}
+        self.m, self.v = ({k: np.zeros(p.size, np.float32) for k, p in self.p.items()} for _ in range(2))
+        self.t = 0
+
+    def check(self, grads, lr=1e-3, decay=None, lr_scales=None, scale=1.0, master=False):
+        o = self.opt
+        self.t += 1
+        got_m, got_v = o.moments()
+        for k, g in grads.items():
+            gg = flat(g)
+            args = dict(beta1=o.beta1, beta2=o.beta2, scale=scale)
+            wd = o.weight_decay if decay is None else decay[k]
+            pn, _, _, bound = oadamw.step64(self.p[k], gg, self.m[k], self.v[k], lr=lr * (lr_scales or {}).get(k, 1.0),
+                                            eps=o.eps, decay=wd, t=self.t, **args)
+            self.m[k], self.v[k] = oadamw.step32(gg, self.m[k], self.v[k], **args)
+            if o.state_bits == 8:
+                self.m[k] = oadamw.values(*oadamw.quantize(self.m[k], self.t, False), False)[:gg.size]
+                self.v[k] = oadamw.values(*oadamw.quantize(self.v[k], self.t, True), True)[:gg.size]
+            np.testing.assert_array_equal(flat(got_m[k]), self.m[k], err_msg=f"m of {k}")
+            np.testing.assert_array_equal(flat(got_v[k]), self.v[k], err_msg=f"v of {k}")
+            p = self.params[k]
+            held = flat(o._views(o.master_slab)[k]) if master else flat(p)
+            dt = F32 if master else p.dtype
+            tol = bound + HALF_STEP[dt] * np.abs(pn) + TINY[dt]
+            err = np.abs(held - pn)
+            assert (err <= tol).all(), (k, (err / np.maximum(tol, 1e-300)).max())
+            if master:
+                np.testing.assert_array_equal(flat(p), flat(torch.from_numpy(held).to(p.dtype)))
+            self.p[k] = held
+        assert o.t == self.t
+        # padding behind every tensor stays zero
+        for slab in o.moment_slabs():
+            total = sum(float(x.double().abs().sum()) for x in o._views(slab).values())
+            assert abs(float(slab.double().abs().sum()) - total) <= 1e-9 * total
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("ptype,gtype,master", [(F32, F32, False), (F32, BF16, False), (BF16, BF16, False),
+                                                (F16, F16, False), (BF16, F32, False), (BF16, BF16, True),
+                                                (F16, F16, True)])
+def test_step_matches_oracle(bits, ptype, gtype, master):
+    shapes = {f"x{i}": (n,) for i, n in enumerate(SIZES)}
+    params = tensors(1, shapes, ptype)
+    lr_scales, decays = {"x0": 3.0, "x5": 0.0, "x11": 0.05}, {"x3": 0.0, "x8": 2.0}
+    opt = FusedAdamW(params, lr=1e-2, weight_decay=0.1, lr_scales=lr_scales, decay_scales=decays, state_bits=bits,
+                     master_weights=master)
+    ref = Reference(opt, params)
+    for s in range(4):
+        grads = tensors(10 + s, shapes, gtype, scale=1e-2, sparse=0.3)
+        assert opt.step(grads) is None
+        ref.check(grads, lr=1e-2, decay={k: 0.1 * decays.get(k, 1.0) for k in shapes}, lr_scales=lr_scales,
+                  master=master)
+
+
+def test_mixed_types_in_one_step_and_grad_scale():
+    shapes = {"a": (33, 5), "b": (2050,), "c": (7, 11, 13), "d": ()}
+    params = {**tensors(1, {"a": shapes["a"], "d": ()}, F32), **tensors(2, {"b": shapes["b"]}, BF16),
+              **tensors(3, {"c": shapes["c"]}, F16)}
+    params = {k: params[k] for k in shapes}
+    opt = FusedAdamW(params, lr=1e-2, state_bits=8)
+    ref = Reference(opt, params)
+    for s in range(3):
+        grads = {k: tensors(20 + s, {k: shapes[k]}, dt, scale=50.0)[k]
+                 for k, dt in zip(shapes, (BF16, F16, F32, F32))}
+        opt.step(grads, grad_scale=1 / 64)
+        ref.check(grads, lr=1e-2, scale=1 / 64)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_strided_rows_leave_their_surroundings(bits):
+    """Columns of one slab (a pool's views), an offset view and strided gradients."""
+    slab = torch.randn(301, 20, device=DEV)
+    back = torch.randn(4000, device=DEV)
+    params = {"q": slab[:, 0:4], "m": slab[:, 4:7], "o": slab[:, 7:8], "s": slab[2:250:2, 9:12], "odd": back[3:3000]}
+    before, before_back = slab.clone(), back.clone()
+    opt = FusedAdamW(params, lr=1e-2, state_bits=bits)
+    ref = Reference(opt, params)
+    gs = torch.randn(301, 24, device=DEV) * 0.01
+    for s in range(3):
+        gs = gs.roll(1, 0) * 1.5
+        wide = torch.randn(2997, 3, device=DEV)
+        grads = {"q": gs[:, 2:6], "m": gs[:, 6:9].contiguous(), "o": gs[:, 9:10], "s": gs[:124, 1:4].t().contiguous().t(),
+                 "odd": wide[:, 1] if s else wide[:, 1].contiguous()}
+        opt.step(grads)
+        ref.check(grads, lr=1e-2)
+    np.testing.assert_array_equal(slab[:, 12:].cpu(), before[:, 12:].cpu())
+    np.testing.assert_array_equal(slab[:, 8].cpu(), before[:, 8].cpu())
+    np.testing.assert_array_equal(slab[1::2, 9:12].cpu(), before[1::2, 9:12].cpu())
+    np.testing.assert_array_equal(slab[250:, 9:12].cpu(), before[250:, 9:12].cpu())
+    np.testing.assert_array_equal(back[:3].cpu(), before_back[:3].cpu())
+    np.testing.assert_array_equal(back[3000:].cpu(), before_back[3000:].cpu())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_broadcast_gradients_and_missing_ones(bits):
+    shapes = {"a": (300,), "b": (40, 9), "c": (3,)}
+    params = {k: p.requires_grad_(True) for k, p in tensors(1, shapes, F32).items()}
+    opt = FusedAdamW(params, state_bits=bits)
+    ref = Reference(opt, params)
+    grads = {"a": torch.full((1,), 0.25, device=DEV).expand(300), "b": torch.randn(9, 40, device=DEV).t()}
+    opt.step(grads)
+    ref.check(grads)
+    before = params["b"]._version
+    params["b"].grad = torch.randn(40, 9, device=DEV)
+    a0 = params["a"].detach().clone()
+    opt.step()  # from .grad; a and c have none
+    ref.check({"b": params["b"].grad})
+    assert params["b"]._version > before and torch.equal(params["a"], a0)
+    params["b"].grad = None
+    assert opt.step() is None and opt.t == 2  # nothing to do
+
+
+@pytest.mark.parametrize("count", [25, 368, 369, 900])
+def test_more_tensors_than_a_table(count):
+    rng = np.random.default_rng(count)
+    shapes = {f"x{i}": (int(n),) for i, n in enumerate(rng.integers(0, 700, count))}
+    params = tensors(1, shapes, F32)
+    opt = FusedAdamW(params, state_bits=8, max_norm=0.5)
+    ref = Reference(opt, params)
+    for s in range(2):
+        grads = tensors(5 + s, shapes, F32, scale=1e-3)
+        norm = opt.step(grads)
+        exact = math.sqrt(sum(float(g.double().square().sum()) for g in grads.values()))
+        assert abs(float(norm) - exact) <= 2.0 ** -24 * 1.01 * exact
+        ref.check(grads, scale=min(1.0, 0.5 / exact))
+
+
+# ---------------------------------------------------------------- norm and clipping
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("scale", [1e-12, 1.0, 0.25, 1e12])
+def test_clip_gradients(dtype, scale):
+    if dtype == F16 and scale != 1.0:
+        scale = {1e-12: 1e-3, 0.25: 0.25, 1e12: 30.0}[scale]
+    shapes = {f"x{i}": (n,) for i, n in enumerate(SIZES + [100_001])}
+    grads = tensors(3, shapes, dtype, scale=scale, sparse=0.2)
+    exact = math.sqrt(sum(float(g.double().square().sum()) for g in grads.values()))
+    before = {k: g.clone() for k, g in grads.items()}
+    # not clipped: the gradients keep their bits
+    norm = clip_gradients(grads, exact * 1.01)
+    assert norm.dtype == F32 and norm.shape == ()
+    if dtype == F16 and scale == 30.0:  # the largest of these pass float16's range: infinities are left
+        assert math.isinf(exact) and math.isinf(float(norm))
+        clip_gradients(grads, 1.0)
+        assert all(torch.equal(grads[k], before[k]) for k in shapes)
+        return
+    assert abs(float(norm) - exact) <= 2.0 ** -24 * 1.01 * exact
+    assert all(torch.equal(grads[k], before[k]) for k in shapes)
+    # clipped, into tensors of every type
+    for out_type in (F32, BF16, F16) if scale == 1.0 else (dtype,):
+        out = {k: torch.full_like(g, 7.0, dtype=out_type) for k, g in grads.items()}
+        clip_gradients(grads, 0.3 * exact, out=out)
+        for k in shapes:
+            want = before[k].double() * 0.3
+            # two float32 roundings (factor, product) and the type's
+            tol = (HALF_STEP[out_type] + 2.0 ** -23 * 1.01) * want.abs() + TINY[out_type] + 2.0 ** -149
+            assert ((out[k].double() - want).abs() <= tol).all(), k
+            assert torch.equal(grads[k], before[k])
+    # in place, the same bits
+    out = {k: torch.empty_like(g) for k, g in grads.items()}
+    clip_gradients(list(grads.values()), 0.3 * exact, out=list(out.values()))
+    clip_gradients(list(grads.values()), 0.3 * exact)
+    assert all(torch.equal(grads[k], out[k]) for k in shapes)
+
+
+def test_clip_strided_and_repeated_gradients():
+    slab = torch.randn(50, 12, device=DEV)
+    same = torch.randn(77, device=DEV)
+    grads = [slab[:, 1:4], slab[:, 5:6], same, same, torch.randn(6, 50, device=DEV).t()]
+    exact = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    rows = torch.zeros(77, 4, device=DEV)
+    out = [torch.zeros(50, 3, device=DEV), torch.zeros(50, 1, device=DEV), rows[:, 0], torch.zeros(77, device=DEV),
+           torch.zeros(50, 6, device=DEV)]
+    norm = clip_gradients(grads, 1.0, out=out)
+    assert abs(float(norm) - exact) <= 2.0 ** -24 * 1.01 * exact
+    for g, o in zip(grads, out):
+        want = g.double() / exact
+        assert ((o.double() - want).abs() <= 2.0 ** -23 * 1.01 * want.abs()).all()
+    assert not rows[:, 1:].any()
+    before = slab.clone()
+    clip_gradients(grads[:2], 1e-3)
+    assert torch.equal(slab[:, 0], before[:, 0]) and torch.equal(slab[:, 4], before[:, 4])
+    assert torch.equal(slab[:, 6:], before[:, 6:]) and not torch.equal(slab[:, 1:4], before[:, 1:4])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_not_finite_gradients_are_left(bad):
+    g = {"a": torch.randn(5000, device=DEV), "b": torch.zeros(0, device=DEV), "c": torch.randn(3, device=DEV)}
+    g["a"][4321] = bad
+    before = {k: x.clone() for k, x in g.items()}
+    norm = float(clip_gradients(g, 0.1))
+    assert not math.isfinite(norm)
+    for k in g:
+        np.testing.assert_array_equal(g[k].cpu(), before[k].cpu())
+    assert float(clip_gradients([torch.zeros(40, device=DEV)], 1.0)) == 0.0
+    assert float(clip_gradients([torch.zeros(0, device=DEV)], 1.0)) == 0.0
+    huge = torch.full((3000,), 1e37, device=DEV)  # squares past float32, the norm (5.5e38) too
+    assert math.isinf(float(clip_gradients([huge], 1.0))) and (huge == 1e37).all()
+    huge[400:] = 0.0  # the norm, 2e38, is in range
+    assert abs(float(clip_gradients([huge], 1e30)) - 2e38) <= 2.0 ** -23 * 2e38
+    # 1e37 itself, the factor and the product are rounded
+    assert ((huge[:400].double() - 5e28).abs() <= 3.01 * 2.0 ** -24 * 5e28).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("kw", [dict(max_norm=1.0), dict(skip_nonfinite=True)])
+def test_step_is_skipped_for_not_finite_gradients(bits, kw):
+    shapes = {"a": (700,), "b": (3000,)}
+    params = tensors(1, shapes, BF16)
+    opt = FusedAdamW(params, state_bits=bits, master_weights=True, **kw)
+    opt.step(tensors(2, shapes, BF16))
+    state = opt.state_dict()
+    before = {k: p.clone() for k, p in params.items()}
+    grads = tensors(3, shapes, BF16)
+    grads["b"][2999] = math.nan
+    assert math.isnan(float(opt.step(grads)))
+    after = opt.state_dict()
+    assert after["t"] == 1
+    for k in ("m", "v", "m_exp", "v_exp", "master"):
+        assert torch.equal(after[k], state[k]), k
+    assert all(torch.equal(params[k], before[k]) for k in shapes)
+    norm = opt.step(tensors(4, shapes, BF16))  # the next step runs
+    assert math.isfinite(float(norm)) and opt.t == 2 and not torch.equal(params["a"], before["a"])
+
+
+def test_skip_alone_does_not_clip():
+    shapes = {"a": (700,)}
+    params = tensors(1, shapes, F32)
+    opt = FusedAdamW(params, skip_nonfinite=True)
+    ref = Reference(opt, params)
+    grads = tensors(2, shapes, F32, scale=100.0)
+    norm = opt.step(grads, grad_scale=-0.5)
+    exact = 0.5 * float(grads["a"].double().norm())
+    assert abs(float(norm) - exact) <= 2.0 ** -24 * 1.01 * exact
+    ref.check(grads, scale=-0.5)
+
+
+def test_not_finite_values_stay_in_their_elements():
+    shapes = {"a": (1000,), "b": (50,)}
+    for bits in (32, 8):
+        params = tensors(1, shapes, F32)
+        opt = FusedAdamW(params, state_bits=bits)
+        grads = tensors(2, shapes, F32)
+        grads["a"][300] = math.inf
+        opt.step(grads)
+        opt.step(tensors(3, shapes, F32))
+        bad = ~torch.isfinite(params["a"]).cpu().numpy()
+        want = np.zeros(1000, bool)
+        if bits == 32:
+            want[300] = True
+        else:
+            want[256:512] = True  # the block's exponent is gone
+        np.testing.assert_array_equal(bad, want)
+        assert torch.isfinite(params["b"]).all()
+
+
+# ---------------------------------------------------------------- the 8-bit form
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_load_moments_matches_oracle(dtype):
+    shapes = {f"x{i}": (n,) for i, n in enumerate(SIZES)}
+    params = tensors(1, shapes, F32)
+    opt = FusedAdamW(params, state_bits=8)
+    m = tensors(2, shapes, dtype, sparse=0.2)
+    v = {k: x.square() for k, x in tensors(3, shapes, dtype, sparse=0.2).items()}
+    if dtype == F32:  # sizes over more than the form's range, in blocks of their own
+        m["x11"][256:512] *= torch.exp(8 * torch.randn(256, device=DEV))
+        v["x11"][512:768] *= torch.exp(30 * torch.randn(256, device=DEV)).clamp(max=1e30)
+        m["x11"][1024:1280] *= 1e-30
+        v["x11"][1280:1536] *= 1e-36
+        m["x11"][1536:1792] *= 1e30
+    opt.load_moments(m, v, t=77)
+    assert opt.t == 77
+    for dt in (F32, BF16):
+        got_m, got_v = opt.moments(dt)
+        for k in shapes:
+            n = m[k].numel()
+            want = oadamw.values(*oadamw.quantize(flat(m[k]), 77, False), False)[:n]
+            np.testing.assert_array_equal(finite(got_m[k]), want, err_msg=k)
+            want = oadamw.values(*oadamw.quantize(flat(v[k]), 77, True), True)[:n]
+            np.testing.assert_array_equal(finite(got_v[k]), want, err_msg=k)
+    # what the form holds is kept, at any step
+    codes = opt.m.clone(), opt.v.clone(), opt.m_exp.clone(), opt.v_exp.clone()
+    opt.load_moments(*opt.moments(), t=1234)
+    live = torch.zeros(opt.slab_elements, dtype=torch.bool, device=DEV)
+    for view in opt._views(live).values():
+        view.fill_(True)
+    for a, b, e in zip(codes[:2], (opt.m, opt.v), codes[2:]):
+        on = live & (e != 255).repeat_interleave(BLOCK)
+        assert torch.equal(a[on], b[on])
+    assert torch.equal(codes[2], opt.m_exp) and torch.equal(codes[3], opt.v_exp)
+
+
+def test_state_dicts():
+    shapes = {"a": (700,), "b": (33, 3)}
+    grads = [tensors(5 + s, shapes, F32) for s in range(4)]
+    runs = []
+    for resume in (False, True):
+        params = tensors(1, shapes, BF16)
+        opt = FusedAdamW(params, state_bits=8, master_weights=True)
+        for s, g in enumerate(grads):
+            if resume and s == 2:
+                d = opt.state_dict()
+                opt = FusedAdamW(params, state_bits=8, master_weights=True)
+                opt.load_state_dict(d)
+            opt.step(g)
+        runs.append((params, opt.state_dict()))
+    for k in shapes:
+        assert torch.equal(runs[0][0][k], runs[1][0][k])
+    for k in ("m", "v", "m_exp", "v_exp", "master"):
+        assert torch.equal(runs[0][1][k], runs[1][1][k])
+    # between the forms: 8 -> 32 -> 8 bits keeps the codes
+    wide = FusedAdamW(tensors(1, shapes, BF16), state_bits=32)
+    wide.load_state_dict(runs[0][1])
+    assert wide.t == 4
+    again = FusedAdamW(tensors(1, shapes, BF16), state_bits=8)
+    again.load_state_dict(wide.state_dict())
+    for a, b in zip(again.moment_slabs(), wide.moment_slabs()):
+        assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="other parameters"):
+        FusedAdamW(tensors(1, {"a": (700,)}, BF16)).load_state_dict(runs[0][1])
+
+
+# ---------------------------------------------------------------- streams, graphs, memory
+@pytest.mark.parametrize("bits,kw", [(32, {}), (8, dict(max_norm=0.3))])
+def test_captured_steps_equal_eager_ones(bits, kw):
+    shapes = {"a": (5000,), "b": (33, 3), "c": (1,)}
+    grads = [tensors(5 + s, shapes, F32) for s in range(6)]
+    lrs = [1e-3 * 0.9 ** s for s in range(6)]
+    eager, graphed = tensors(1, shapes, F32), tensors(1, shapes, F32)
+    lr = torch.zeros(1, device=DEV)
+    a = FusedAdamW(eager, state_bits=bits, lr=lr, **kw)
+    for g, x in zip(grads, lrs):
+        lr.fill_(x)
+        a.step(g)
+    lr2 = torch.full((), lrs[0], device=DEV)
+    b = FusedAdamW(graphed, state_bits=bits, lr=lr2, **kw)
+    static = {k: g.clone() for k, g in grads[0].items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b.step(static)  # on another stream than the tensors' own
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.step(static)
+    assert b.t == 1
+    for g, x in list(zip(grads, lrs))[1:]:
+        for k in shapes:
+            static[k].copy_(g[k])
+        lr2.fill_(x)
+        graph.replay()
+    assert a.t == b.t == 6
+    assert all(torch.equal(eager[k], graphed[k]) for k in shapes)
+    for x, y in zip(a.moment_slabs(), b.moment_slabs()):
+        assert torch.equal(x, y)
+
+
+def test_two_captured_clips_do_not_share_workspace():
+    one, two = torch.randn(200_000, device=DEV), torch.randn(300_000, device=DEV)
+    outs = torch.empty_like(one), torch.empty_like(two)
+    want = [clip_gradients([x], 1.0, out=[torch.empty_like(x)]) for x in (one, two)]
+    graphs = []
+    for x, o in zip((one, two), outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            norm = clip_gradients([x], 1.0, out=[o])
+        graphs.append((g, norm))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for w, x, o, (_, norm) in zip(want, (one, two), outs, graphs):
+        assert torch.equal(w, norm)
+        assert abs(float(o.double().norm()) - 1.0) < 1e-6
+
+
+def test_replaced_parameter_memory():
+    params = {"a": torch.randn(100, device=DEV), "b": torch.randn(30, device=DEV)}
+    opt = FusedAdamW(params)
+    ref = Reference(opt, params)
+    params["a"].data = params["a"].data.clone()
+    grads = tensors(2, {"a": (100,), "b": (30,)}, F32)
+    opt.step(grads)
+    ref.check(grads)
+    params["a"].data = torch.randn(50, device=DEV)
+    with pytest.raises(ValueError):
+        opt.step({"b": grads["b"]})
+
+
+def test_elements_past_32_bits():
+    n = (1 << 31) + 4101
+    p = torch.zeros(n, dtype=BF16, device=DEV)
+    g = torch.zeros(n, dtype=BF16, device=DEV)
+    spots = [slice(0, 600), slice((1 << 31) - 300, (1 << 31) + 300), slice(n - 600, n)]
+    gen = torch.Generator().manual_seed(0)
+    for s in spots:
+        p[s] = torch.randn(600, generator=gen).to(BF16).to(DEV)
+        g[s] = torch.randn(600, generator=gen).to(BF16).to(DEV)
+    p0 = [flat(p[s]) for s in spots]
+    opt = FusedAdamW({"p": p}, lr=0.1, state_bits=8, max_norm=1.0)
+    norm = float(opt.step({"p": g}))
+    exact = math.sqrt(sum(float(g[s].double().square().sum()) for s in spots))
+    assert abs(norm - exact) <= 2.0 ** -24 * 1.01 * exact
+    m, v = opt.moments(BF16)
+    for s, before in zip(spots, p0):
+        lo = s.start // BLOCK * BLOCK
+        hi = min(n, -(-s.stop // BLOCK) * BLOCK)
+        gg, zero = flat(g[lo:hi]), np.zeros(hi - lo, np.float32)
+        mm, vv = oadamw.step32(gg, zero, zero, beta1=0.9, beta2=0.999, scale=1.0 / exact)
+        np.testing.assert_array_equal(flat(m["p"][lo:hi]), oadamw.values(*oadamw.quantize(mm, 1, False, first=lo), False)[:hi - lo])
+        np.testing.assert_array_equal(flat(v["p"][lo:hi]), oadamw.values(*oadamw.quantize(vv, 1, True, first=lo), True)[:hi - lo])
+        pn, _, _, bound = oadamw.step64(before, flat(g[s]), np.zeros(600), np.zeros(600), lr=0.1, beta1=0.9, beta2=0.999,
+                                        eps=1e-8, decay=0.01, t=1, scale=1.0 / exact)
+        assert (np.abs(flat(p[s]) - pn) <= bound + 2.0 ** -8 * np.abs(pn)).all()
+
+
+# ---------------------------------------------------------------- refusals with device tensors
+def test_refusals_on_the_device():
+    params = {"a": torch.zeros(8, device=DEV), "b": torch.zeros(3, device=DEV)}
+    with pytest.raises(ValueError, match="one device"):
+        FusedAdamW({"a": params["a"], "b": torch.zeros(3)})
+    with pytest.raises(ValueError, match="lr"):
+        FusedAdamW(params, lr=-1.0)
+    with pytest.raises(ValueError, match="tensor lr"):
+        FusedAdamW(params, lr=torch.zeros(2, device=DEV))
+    with pytest.raises(ValueError, match="tensor lr"):
+        FusedAdamW(params, lr=torch.zeros(1))
+    with pytest.raises(ValueError, match="max_norm"):
+        FusedAdamW(params, max_norm=0.0)
+    opt = FusedAdamW(params)
+    g = {"a": torch.ones(8, device=DEV), "b": torch.ones(3, device=DEV)}
+    with pytest.raises(ValueError, match="shape"):
+        opt.step({**g, "b": torch.ones(4, device=DEV)})
+    with pytest.raises(ValueError, match="float64"):
+        opt.step({**g, "b": g["b"].double()})
+    with pytest.raises(ValueError, match="must be on"):
+        opt.step({**g, "b": torch.ones(3)})
+    with pytest.raises(ValueError, match="sparse"):
+        opt.step({**g, "b": g["b"].to_sparse()})
+    with pytest.raises(ValueError, match="no parameter named"):
+        opt.step({"z": g["a"]})
+    with pytest.raises(ValueError, match="grad_scale"):
+        opt.step(g, grad_scale=math.inf)
+    with pytest.raises(ValueError, match="exactly"):
+        opt.load_moments({"a": g["a"]}, {"a": g["a"]})
+    with pytest.raises(ValueError, match="shape"):
+        opt.load_moments({**g, "a": g["b"]}, g)
+    with pytest.raises(ValueError, match="step count"):
+        opt.load_moments(g, g, t=-1)
+    with pytest.raises(ValueError, match="float32 or bfloat16"):
+        FusedAdamW(params, state_bits=8).moments(F16)
+    with pytest.raises(ValueError, match="one device"):
+        clip_gradients([g["a"], torch.zeros(3)], 1.0)
+    assert not params["a"].any() and opt.t == 0
+
+
+# ---------------------------------------------------------------- as they are used
+@pytest.mark.parametrize("bits", [32, 8])
+def test_training_a_scene_with_an_exposure_beside_it(bits):
+    """Autograd through the rasterizer, slab views of a pool and a small exposure
+    tensor in one optimizer, clipped: every step's update is the oracle's for the
+    step's own gradients, and the exposure's gradient agrees with differences."""
+    wl = synthetic.WORKLOADS["tiny-3k"]
+    g = synthetic.make_gaussians(wl, seed=0, n=400)
+    views, K = synthetic.make_cameras(wl, seed=2)
+    al = PointerStableChunkedAllocator(500, sh_degree=0, device=torch.device(DEV, 0))
+    al.set_initial_gaussians(g)
+    names = ("means", "quats", "scales", "opacities", "sh0")
+    pools = {k: al.physical_pools[k][:400] for k in names}
+    leaves = {k: p.detach().requires_grad_(True) for k, p in pools.items()}
+    leaves["exposure"] = torch.eye(3, 4, device=DEV).requires_grad_(True)
+    opt = FusedAdamW(leaves, lr=1e-2, weight_decay=0.0, max_norm=1e-3, state_bits=bits)
+    ref = Reference(opt, leaves)
+    target = torch.rand(wl.height, wl.width, 3, device=DEV)
+
+    def loss_of(step):
+        vm = views[step]
+        args = [leaves[k].contiguous() for k in names]
+        ids = frustum_culling_mlx(args[0].detach(), None, None, vm, K, wl.width, wl.height,
+                                  opacities=args[3].detach())
+        C, _ = rasterize_gaussians_mlx(*args[:4], args[4][ids.long()], vm, K, wl.width, wl.height, ids,
+                                       render_width=wl.width, render_height=wl.height)
+        C = C.reshape(wl.height, wl.width, 3) @ leaves["exposure"][:, :3].t() + leaves["exposure"][:, 3]
+        return (C - target).square().mean()
+
+    for step in range(3):
+        for p in leaves.values():
+            p.grad = None
+        loss_of(step).backward()
+        grads = {k: p.grad for k, p in leaves.items()}
+        exact = math.sqrt(sum(float(x.double().square().sum()) for x in grads.values()))
+        norm = opt.step()
+        assert abs(float(norm) - exact) <= 2.0 ** -24 * 1.01 * exact
+        ref.check(grads, lr=1e-2, scale=min(1.0, 1e-3 / exact))
+    with torch.no_grad():
+        e = leaves["exposure"]
+        leaves["exposure"].grad = None
+    loss_of(0).backward()
+    with torch.no_grad():
+        for r, c in ((0, 0), (1, 3)):
+            x = float(e[r, c])
+            h = 1e-2  # the loss is quadratic in the exposure: a central difference has no error of its own
+            e[r, c] = x + h
+            up = float(loss_of(0).double())
+            e[r, c] = x - h
+            down = float(loss_of(0).double())
+            e[r, c] = x
+            # float32 losses of order 1 differ by 2 h |grad|: their own rounding enters over 2 h
+            assert abs((up - down) / (2 * h) - float(e.grad[r, c])) <= 16 * 2.0 ** -24 * max(up, down) / (2 * h) + 1e-3 * abs(float(e.grad[r, c]))
+
+
+def test_beside_the_pooled_adam():
+    """Without weight decay the step is the pooled Adam's formula: both move a
+    group alike, up to float32 rounding of the step."""
+    shapes = {"means": (500, 3)}
+    p = tensors(1, shapes, F32)
+    q = {k: x.clone() for k, x in p.items()}
+    opt, pooled = FusedAdamW(p, lr=1e-2, weight_decay=0.0, eps=1e-15), FusedMLXAdam(lr=1e-2, eps=1e-15)
+    m, v = ({k: torch.zeros_like(x) for k, x in q.items()} for _ in range(2))
+    for s in range(3):
+        g = tensors(7 + s, shapes, F32)
+        before = {k: x.clone() for k, x in p.items()}
+        opt.step(g)
+        q, m, v = pooled.step(q, g, m, v)
+        got_m, got_v = opt.moments()
+        for k in shapes:
+            assert torch.equal(got_m[k], m[k]) and torch.equal(got_v[k], v[k])
+            # each side: at most 16 roundings of the step and 2 of the parameter, a step
+            tol = (s + 1) * 2.0 ** -24 * (32 * 1e-2 * 8 + 4 * before[k].abs())
+            assert ((p[k] - q[k]).abs() <= tol).all()
