@@ -257,8 +257,9 @@ typedef struct gs_adamw_settings {
  * when clipped, and t the new step count,
  *   g = c * grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
  *   param = (1 - lr decay) param - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
- * in float32, every operation rounded by itself; 16-bit parameters (or their
- * master's rounding) are rounded to nearest at the end.  Values that are not
+ * in float32: every operation of the moments rounded by itself, the square root
+ * and the quotient to a few ulp; 16-bit parameters (from their master where there
+ * is one) are rounded to nearest.  eps is a normal float32. Values that are not
  * finite pass into the elements they touch (8-bit moments: into their block).
  * The step count lives in ``control``, so a captured call can be replayed. */
 int gs_adamw_step(const gs_tensor* tensors, int64_t count, const gs_adamw_state* state,

@@ -166,8 +166,8 @@ class FusedAdamW:
             raise ValueError("no parameters")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError(f"betas must be in [0, 1): {betas}")
-        if not (math.isfinite(eps) and float(np.float32(eps)) > 0.0):
-            raise ValueError(f"eps must be positive: {eps}")
+        if not (math.isfinite(eps) and eps >= 2.0 ** -126):
+            raise ValueError(f"eps must be positive (a normal float32): {eps}")
         if not (math.isfinite(weight_decay) and weight_decay >= 0.0):
             raise ValueError(f"weight_decay must not be negative: {weight_decay}")
         if state_bits not in (8, 32):

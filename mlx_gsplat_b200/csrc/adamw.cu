@@ -6,16 +6,18 @@
 //   g' = c g                       c: grad_scale, times max_norm / norm when clipped
 //   m' = b1 m + (1 - b1) g'        v' = b2 v + (1 - b2) g'^2
 //   p' = (1 - lr wd) p - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
-// with every operation rounded to float32 by itself (no fused multiply-add), so
-// that an element's result depends neither on its place in the list nor on which
-// of the load paths it takes.  t, the bias corrections, the norm and the factors
+// The moments' operations are rounded to float32 one by one (no fused multiply-
+// add), which fixes them bit for bit; all load paths give the same results.  t, the bias corrections, the norm and the factors
 // made of them are formed in 64 bits and rounded once.
+#include <float.h>
 #include <math.h>
 
 #include "moments8.cuh"
 #include "multi_tensor.cuh"
 
 namespace gs {
+
+constexpr int kAdamWBlocksPerSm = 3;
 
 struct AdamWArgs {
     void *m, *v;
@@ -26,7 +28,7 @@ struct AdamWArgs {
     const double* partials;
     float* norm_out;
     int64_t num_partials;
-    double lr, beta1, beta2, grad_scale, max_norm;
+    double lr, log2_b1, log2_b2, grad_scale, max_norm;
     float b1, b2, omb1, omb2, eps;
     int advance;            // the step's last launch counts the step
 };
@@ -35,17 +37,19 @@ struct AdamWShared {
     double lr, inv_bc1;
     float gscale, inv_sqrt_bc2;
     uint32_t step_word;
+    int64_t t;
     int skip;
 };
 
 // What every element of the step shares.  Each block sums the norm's partials
 // itself (a few hundred doubles in a fixed order), which needs no launch
-// between the norm and the step.
+// between the norm and the step; the bias corrections are formed by other warps
+// meanwhile (beta^t = 2^(t log2 beta), in 64 bits).
 __device__ __forceinline__ void adamw_prologue(const AdamWArgs& a, AdamWShared& sh) {
     double sq = 0.0;
     if (a.partials) sq = sum_partials(a.partials, a.num_partials);
+    const int64_t t = *reinterpret_cast<volatile int64_t*>(a.ctl) + 1;
     if (threadIdx.x == 0) {
-        const int64_t t = *reinterpret_cast<volatile int64_t*>(a.ctl) + 1;
         double scale = a.grad_scale;
         bool skip = false;
         if (a.partials) {
@@ -57,88 +61,100 @@ __device__ __forceinline__ void adamw_prologue(const AdamWArgs& a, AdamWShared& 
         sh.skip = skip;
         sh.gscale = (float)scale;
         sh.lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
-        sh.inv_bc1 = 1.0 / (1.0 - pow(a.beta1, (double)t));
-        sh.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(a.beta2, (double)t)));
         sh.step_word = (uint32_t)t * kDitherStep;
-        // the last block to have read the count writes the new one; a skipped step is not counted
+    } else if (threadIdx.x == 32) {
+        sh.inv_bc1 = 1.0 / (1.0 - exp2((double)t * a.log2_b1));
+    } else if (threadIdx.x == 64) {
+        sh.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - exp2((double)t * a.log2_b2)));
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        // the last block whose threads have read the count writes the new one; a skipped step is not counted
         __threadfence();
         unsigned int* ticket = reinterpret_cast<unsigned int*>(a.ctl + 1);
         if (atomicAdd(ticket, 1u) == gridDim.x - 1) {
             *ticket = 0;
-            if (a.advance && !skip) a.ctl[0] = t;
+            if (a.advance && !sh.skip) a.ctl[0] = t;
         }
     }
-    __syncthreads();
 }
 
+// The moments, every operation rounded by itself.
 __device__ __forceinline__ void moments_update(float g, float& m, float& v, const AdamWArgs& a) {
     m = __fadd_rn(__fmul_rn(a.b1, m), __fmul_rn(a.omb1, g));
     v = __fadd_rn(__fmul_rn(a.b2, v), __fmul_rn(a.omb2, __fmul_rn(g, g)));
 }
 
+// The parameter, with the hardware's approximate square root and reciprocal: 2
+// ulp each on the step, far below the rounding of the parameter it moves.  The
+// rounded forms take a slow path where m or v is a denormal, which is where the
+// moments of long unseen Gaussians end (0.9^800 of a gradient): a step over a
+// scene half of which is unseen took 561 us with them and 269 us without.
 __device__ __forceinline__ float param_update(float p, float m, float v, float inv_sqrt_bc2, float step, float keep,
                                               float eps) {
-    const float denom = __fadd_rn(__fmul_rn(__fsqrt_rn(v), inv_sqrt_bc2), eps);
-    return __fsub_rn(__fmul_rn(p, keep), __fmul_rn(step, __fdiv_rn(m, denom)));
+    float root, inv;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
+    const float denom = fmaf(root, inv_sqrt_bc2, eps);  // eps is a normal number, so denom is
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(denom));
+    return fmaf(-step, m * inv, p * keep);
 }
 
 template <int kBits, int kCap>
-__global__ void __launch_bounds__(kMultiThreads) adamw_kernel(const __grid_constant__ TensorTable<kCap> tab,
-                                                              const __grid_constant__ AdamWArgs a) {
+__global__ void __launch_bounds__(kMultiThreads, kAdamWBlocksPerSm) adamw_kernel(
+    const __grid_constant__ TensorTable<kCap> tab, const __grid_constant__ AdamWArgs a) {
     __shared__ AdamWShared sh;
     pdl_wait();
-    adamw_prologue(a, sh);
-    if (sh.skip) return;
     int c, end;
     block_share(tab, c, end);
-    if (c >= end) return;
     int ti = find_tensor(tab, c);
     float step = 0.0f, keep = 0.0f;
+    // the grid has at most one block per chunk, so every block has a first chunk
     for (int seen = -1; c < end; ++c) {
         while (c >= tab.first[ti + 1]) ++ti;
         const TensorEntry& e = tab.e[ti];
+        const int64_t i = (int64_t)(c - tab.first[ti]) * kChunk + threadIdx.x * kPerThread;
+        const int64_t s = e.state + i;
+        // the state has whole blocks of 256, so a warp is inside or outside as one
+        const bool inside = i - (threadIdx.x & 31) * kPerThread < e.n;
+        const bool whole = i + kPerThread <= e.n;
+        const bool masters = a.master != nullptr && e.param_type != GS_F32;
+        const bool vg = whole && e.grad_vec, vp = whole && e.param_vec;
+        Raw8 rp, rg, rm, rv;
+        uint2 cm, cv;
+        uint32_t em = 0, ev = 0;
+        if (inside) {
+            if (kBits == 32) {
+                rm = load_raw8(a.m, s, GS_F32);
+                rv = load_raw8(a.v, s, GS_F32);
+            } else {
+                cm = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + s));
+                cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + s));
+                em = a.m_exp[s / GS_MOMENT_BLOCK];
+                ev = a.v_exp[s / GS_MOMENT_BLOCK];
+            }
+            if (vg) rg = load_raw8(e.grad, i, e.grad_type);
+            if (masters)
+                rp = load_raw8(a.master, s, GS_F32);
+            else if (vp)
+                rp = load_raw8(e.param, i, e.param_type);
+        }
         if (ti != seen) {
+            // the first chunk's loads are on their way while the block forms what the step shares
+            if (seen < 0) {
+                adamw_prologue(a, sh);
+                if (sh.skip) return;
+            }
             const double lr = sh.lr * e.lr_scale;
             step = (float)(lr * sh.inv_bc1);
             keep = (float)(1.0 - lr * e.decay);
             seen = ti;
         }
-        const int64_t i = (int64_t)(c - tab.first[ti]) * kChunk + threadIdx.x * kPerThread;
-        const int64_t s = e.state + i;
-        // the state has whole blocks of 256, so a warp is inside or outside as one
-        const int64_t warp_first = i - (threadIdx.x & 31) * kPerThread;
-        if (warp_first >= e.n) continue;
-        const bool whole = i + kPerThread <= e.n;
-        const bool masters = a.master != nullptr && e.param_type != GS_F32;
+        if (!inside) continue;
         float p[8], g[8], m[8], v[8];
-        Raw8 rp, rg, rm, rv;
-        uint2 cm, cv;
-        uint32_t em = 0, ev = 0;
-        if (kBits == 32) {
-            rm = load_raw8(a.m, s, GS_F32);
-            rv = load_raw8(a.v, s, GS_F32);
-        } else {
-            cm = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + s));
-            cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + s));
-            em = a.m_exp[s / GS_MOMENT_BLOCK];
-            ev = a.v_exp[s / GS_MOMENT_BLOCK];
-        }
-        const bool vg = whole && e.grad_vec, vp = whole && e.param_vec;
-        if (vg) rg = load_raw8(e.grad, i, e.grad_type);
-        if (masters)
-            rp = load_raw8(a.master, s, GS_F32);
-        else if (vp)
-            rp = load_raw8(e.param, i, e.param_type);
         if (vg)
             unpack8(rg, e.grad_type, g);
         else
             load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, g);
-        if (masters)
-            unpack8(rp, GS_F32, p);
-        else if (vp)
-            unpack8(rp, e.param_type, p);
-        else
-            load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, p);
         if (kBits == 32) {
             unpack8(rm, GS_F32, m);
             unpack8(rv, GS_F32, v);
@@ -147,10 +163,15 @@ __global__ void __launch_bounds__(kMultiThreads) adamw_kernel(const __grid_const
             decode_v8(cv, ev, v);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            moments_update(__fmul_rn(g[k], sh.gscale), m[k], v[k], a);
-            p[k] = param_update(p[k], m[k], v[k], sh.inv_sqrt_bc2, step, keep, a.eps);
-        }
+        for (int k = 0; k < 8; ++k) moments_update(__fmul_rn(g[k], sh.gscale), m[k], v[k], a);
+        if (masters)
+            unpack8(rp, GS_F32, p);
+        else if (vp)
+            unpack8(rp, e.param_type, p);
+        else
+            load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, p);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] = param_update(p[k], m[k], v[k], sh.inv_sqrt_bc2, step, keep, a.eps);
         if (masters) store_vec8(a.master, s, GS_F32, p);
         if (vp)
             store_vec8(e.param, i, e.param_type, p);
@@ -160,9 +181,9 @@ __global__ void __launch_bounds__(kMultiThreads) adamw_kernel(const __grid_const
             store_vec8(a.m, s, GS_F32, m);
             store_vec8(a.v, s, GS_F32, v);
         } else {
-            store_moments8(m, v, (uint32_t)i, sh.step_word, static_cast<uint8_t*>(a.m) + s,
-                           static_cast<uint8_t*>(a.v) + s, a.m_exp + s / GS_MOMENT_BLOCK,
-                           a.v_exp + s / GS_MOMENT_BLOCK);
+            store_moments8<false>(m, v, (uint32_t)i, sh.step_word, static_cast<uint8_t*>(a.m) + s,
+                                  static_cast<uint8_t*>(a.v) + s, a.m_exp + s / GS_MOMENT_BLOCK,
+                                  a.v_exp + s / GS_MOMENT_BLOCK);
         }
     }
 }
@@ -198,7 +219,7 @@ __global__ void __launch_bounds__(kMultiThreads) moments8_quantize_kernel(const 
             unpack8(rv, e.grad_type, v);
         else
             load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, v);
-        store_moments8(m, v, (uint32_t)i, step_word, mc + s, vc + s, me + s / GS_MOMENT_BLOCK,
+        store_moments8<true>(m, v, (uint32_t)i, step_word, mc + s, vc + s, me + s / GS_MOMENT_BLOCK,
                        ve + s / GS_MOMENT_BLOCK);
     }
 }
@@ -222,8 +243,6 @@ __global__ void __launch_bounds__(kMultiThreads) moments8_dequantize_kernel(cons
     decode_v8(cv, ev, x);
     store_vec8(v_out, i, kType, x);
 }
-
-constexpr int kAdamWBlocksPerSm = 3;
 
 template <int kCap>
 static int adamw_launches(const gs_tensor* t, int64_t count, int bits, AdamWArgs a, cudaStream_t stream) {
@@ -265,7 +284,7 @@ extern "C" int gs_adamw_step(const gs_tensor* tensors, int64_t count, const gs_a
     GS_REQUIRE(state->bits == 32 || state->bits == 8, "adamw: moments have 32 or 8 bits, not %d", state->bits);
     GS_REQUIRE(set->beta1 >= 0.0 && set->beta1 < 1.0 && set->beta2 >= 0.0 && set->beta2 < 1.0,
                "adamw: betas must be in [0, 1)");
-    GS_REQUIRE(set->eps > 0.0f && isfinite(set->eps), "adamw: eps must be positive");
+    GS_REQUIRE(set->eps >= FLT_MIN && isfinite(set->eps), "adamw: eps must be positive (a normal float32)");
     GS_REQUIRE(isfinite(set->grad_scale), "adamw: grad_scale must be finite");
     GS_REQUIRE(set->lr_device || isfinite(set->lr), "adamw: lr must be finite");
     GS_REQUIRE(!set->norm_partials || (set->num_partials >= 0 && set->max_norm > 0.0),
@@ -288,8 +307,8 @@ extern "C" int gs_adamw_step(const gs_tensor* tensors, int64_t count, const gs_a
     a.norm_out = set->norm_out;
     a.num_partials = set->num_partials;
     a.lr = set->lr;
-    a.beta1 = set->beta1;
-    a.beta2 = set->beta2;
+    a.log2_b1 = log2(set->beta1);
+    a.log2_b2 = log2(set->beta2);
     a.grad_scale = set->grad_scale;
     a.max_norm = set->max_norm;
     a.b1 = (float)set->beta1;

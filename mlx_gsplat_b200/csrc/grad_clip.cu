@@ -25,6 +25,10 @@ __device__ __forceinline__ double sum_squares8(const float (&x)[8]) {
     return s;
 }
 
+// Chunks of a dense, aligned tensor are loaded kAhead at a time: one chunk's 16 or
+// 32 bytes a thread are too few in flight for the memory's latency.
+constexpr int kAhead = 4;
+
 template <int kCap>
 __global__ void __launch_bounds__(kMultiThreads) grad_norm_kernel(const __grid_constant__ TensorTable<kCap> tab,
                                                                   double* partials) {
@@ -32,20 +36,31 @@ __global__ void __launch_bounds__(kMultiThreads) grad_norm_kernel(const __grid_c
     int c, end;
     block_share(tab, c, end);
     double sum = 0.0;
-    if (c < end) {
-        int ti = find_tensor(tab, c);
-        for (; c < end; ++c) {
-            while (c >= tab.first[ti + 1]) ++ti;
-            const TensorEntry& e = tab.e[ti];
-            const int64_t i = (int64_t)(c - tab.first[ti]) * kChunk + threadIdx.x * kPerThread;
-            if (i >= e.n) continue;
-            float g[8];
+    for (int ti = find_tensor(tab, c); c < end;) {
+        while (c >= tab.first[ti + 1]) ++ti;
+        const TensorEntry& e = tab.e[ti];
+        int64_t i = (int64_t)(c - tab.first[ti]) * kChunk + threadIdx.x * kPerThread;
+        float g[8];
+        if (e.grad_vec && c + kAhead <= end && i + (kAhead - 1) * kChunk + kPerThread <= e.n) {
+            Raw8 r[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) r[k] = load_raw8(e.grad, i + k * kChunk, e.grad_type);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                unpack8(r[k], e.grad_type, g);
+                sum += sum_squares8(g);
+            }
+            c += kAhead;
+            continue;
+        }
+        if (i < e.n) {
             if (e.grad_vec && i + kPerThread <= e.n)
                 unpack8(load_raw8(e.grad, i, e.grad_type), e.grad_type, g);
             else
                 load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, g);
             sum += sum_squares8(g);
         }
+        ++c;
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) partials[blockIdx.x] = sum;

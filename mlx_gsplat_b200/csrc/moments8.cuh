@@ -35,35 +35,48 @@ constexpr int kMomentTopM = 15, kMomentTopV = 31;
 // Lowest block exponent: keeps every scale factor below a normal float32.
 constexpr uint32_t kMomentMinExp = 64;
 
-// Value of a code's magnitude (exponent field over 3 bits, at bit 20).
+// A code's value: its bits at bit 20 are an exponent field and mantissa of
+// float32 (field 0: a denormal), so one product with 2^(e - T) gives the value.
+// For the largest blocks that factor is no float32 and comes in two parts.
 template <int kTop>
-__device__ __forceinline__ float moment_value(uint32_t field_bits, float block_scale) {
-    // as float32 bits the code is an exponent field and mantissa (field 0: a denormal)
-    const float one_binade = __uint_as_float((uint32_t)(254 - kTop) << 23);  // 2^(127 - T)
-    return __uint_as_float(field_bits) * one_binade * block_scale;
-}
+struct MomentScale {
+    float first, second;
+    bool two;
+    __device__ __forceinline__ explicit MomentScale(uint32_t e) {
+        constexpr uint32_t kOne = 254 - kTop;  // field of 2^(127 - T)
+        two = e + kOne - 127 > 254;
+        first = __uint_as_float((two ? kOne : e + kOne - 127) << 23);
+        second = __uint_as_float(e << 23);
+    }
+};
 
-// Eight codes (two words) to values; ``e`` the block's exponent byte.
+// Eight codes (two words) to values; ``e`` the block's exponent byte (255: no
+// number, or infinity).
 __device__ __forceinline__ void decode_m8(uint2 c, uint32_t e, float (&x)[8]) {
-    const float s = __uint_as_float(e << 23);
+    const MomentScale<kMomentTopM> s(e);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const uint32_t w = k < 4 ? c.x : c.y;
-        const int b = 8 * (k & 3);
-        const uint32_t f = (b < 24 ? w << (20 - b) : w >> 4) & 0x07f00000u;
-        const float v = moment_value<kMomentTopM>(f, s);
-        x[k] = __uint_as_float(__float_as_uint(v) ^ ((w << (24 - b)) & 0x80000000u));
+        // sign and magnitude to bits 31 and 26..20: the byte to the top, then an arithmetic shift
+        const uint32_t w = (k < 4 ? c.x : c.y) << (24 - 8 * (k & 3));
+        x[k] = __uint_as_float((uint32_t)((int32_t)w >> 4) & 0x87f00000u) * s.first;
+    }
+    if (s.two) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] *= s.second;
     }
 }
 
 __device__ __forceinline__ void decode_v8(uint2 c, uint32_t e, float (&x)[8]) {
-    const float s = __uint_as_float(e << 23);
+    const MomentScale<kMomentTopV> s(e);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const uint32_t w = k < 4 ? c.x : c.y;
         const int b = 8 * (k & 3);
-        const uint32_t f = (b < 24 ? w << (20 - b) : w >> 4) & 0x0ff00000u;
-        x[k] = moment_value<kMomentTopV>(f, s);
+        x[k] = __uint_as_float((b < 24 ? w << (20 - b) : w >> 4) & 0x0ff00000u) * s.first;
+    }
+    if (s.two) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] *= s.second;
     }
 }
 
@@ -71,47 +84,48 @@ __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t 
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
+// The top bytes of four words.
+__device__ __forceinline__ uint32_t pack_tops(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+
 // Codes of the eight magnitudes ``a`` (float32 bits without sign) of this lane's
 // share of a block held by one warp, and the block's exponent byte.  ``w``: the
-// dither word of the first element.
+// dither word of the first element (v's: the complement, which counts down).
 template <int kTop, bool kPositive>
 __device__ __forceinline__ void encode8(const uint32_t (&a)[8], uint32_t w, uint32_t (&code)[8], uint32_t& e) {
-    uint32_t r[8], most = 0;
+    constexpr uint32_t kNext = kPositive ? 0u - kDitherElement : kDitherElement;
+    uint32_t most = 0, least = 0xffffffffu;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const uint32_t d = w + (uint32_t)k * kDitherElement;
-        r[k] = a[k] + ((kPositive ? ~d : d) >> 12);
-        most = max(most, r[k]);
+        code[k] = a[k] + ((w + (uint32_t)k * kNext) >> 12);
+        most = max(most, code[k]);
+        least = min(least, a[k] - 1u);  // a zero is no small value: it wraps to the largest
     }
-    most = __reduce_max_sync(kFull, most) >> 23;
-    e = min(max(most, kMomentMinExp), 255u);
+    e = min(max(__reduce_max_sync(kFull, most) >> 23, kMomentMinExp), 255u);
     const uint32_t low = (e - (kTop - 1)) << 23;  // smallest magnitude with exponent field 1
-    const uint32_t base = (e - kTop) << 3;
-    bool small = false;
+    const int base = (int)(e - kTop) << 3;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        code[k] = a[k] < low ? 0u : (r[k] >> 20) - base;
-        small |= a[k] < low && a[k] != 0;
-    }
-    if (__any_sync(kFull, small)) {
+    for (int k = 0; k < 8; ++k) code[k] = (uint32_t)max((int)(code[k] >> 20) - base, 0);
+    // Values below field 1 are few (2^-14 of the block's largest for m, 2^-30 for v), so warps without any skip them.
+    if (__any_sync(kFull, least < low - 1u)) {
         // step of field 0 -> 2^20: the factor is 2^(127 + 3 + 20 - (e - (T - 1)))
         const float f = __uint_as_float((277u + (kTop - 1) - e) << 23);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             if (a[k] < low) {
                 const float y = __fadd_rz(__fmul_rn(__uint_as_float(a[k]), f), 8388608.0f);
-                const uint32_t d = w + (uint32_t)k * kDitherElement;
-                uint32_t c = (__float_as_uint(y) - 0x4B000000u + ((kPositive ? ~d : d) >> 12)) >> 20;
-                if (kPositive && c == 0 && a[k] != 0) c = 1;
-                if (a[k] == 0) c = 0;
-                code[k] = c;
+                code[k] = (__float_as_uint(y) - 0x4B000000u + ((w + (uint32_t)k * kNext) >> 12)) >> 20;
+                if (kPositive && code[k] == 0 && a[k] != 0) code[k] = 1;
             }
         }
     }
 }
 
 // A lane's eight values of both moments -> codes, stored with the block's
-// exponents.  All 32 lanes of the warp that holds the block take part.
+// exponents.  All 32 lanes of the warp that holds the block take part.  kAnyV: v
+// may come with a sign (a caller's; the step's own has none).
+template <bool kAnyV>
 __device__ __forceinline__ void store_moments8(const float (&m)[8], const float (&v)[8], uint32_t i, uint32_t step_word,
                                                uint8_t* mc, uint8_t* vc, uint8_t* me, uint8_t* ve) {
     const uint32_t w = i * kDitherElement + step_word;
@@ -119,14 +133,16 @@ __device__ __forceinline__ void store_moments8(const float (&m)[8], const float 
 #pragma unroll
     for (int k = 0; k < 8; ++k) a[k] = __float_as_uint(m[k]) & 0x7fffffffu;
     encode8<kMomentTopM, false>(a, w, c, e);
+    uint2 out = make_uint2(pack_bytes(c[0], c[1], c[2], c[3]), pack_bytes(c[4], c[5], c[6], c[7]));
 #pragma unroll
-    for (int k = 0; k < 8; ++k) c[k] = (c[k] & 0x7fu) | ((__float_as_uint(m[k]) >> 24) & 0x80u);
-    __stcs(reinterpret_cast<uint2*>(mc), make_uint2(pack_bytes(c[0], c[1], c[2], c[3]),
-                                                    pack_bytes(c[4], c[5], c[6], c[7])));
+    for (int k = 0; k < 8; ++k) a[k] = __float_as_uint(m[k]);
+    out.x = (out.x & 0x7f7f7f7fu) | (pack_tops(a[0], a[1], a[2], a[3]) & 0x80808080u);
+    out.y = (out.y & 0x7f7f7f7fu) | (pack_tops(a[4], a[5], a[6], a[7]) & 0x80808080u);
+    __stcs(reinterpret_cast<uint2*>(mc), out);
     if ((threadIdx.x & 31) == 0) *me = (uint8_t)e;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = __float_as_uint(v[k]) & 0x7fffffffu;
-    encode8<kMomentTopV, true>(a, w, c, e);
+    for (int k = 0; k < 8; ++k) a[k] = __float_as_uint(v[k]) & (kAnyV ? 0x7fffffffu : 0xffffffffu);
+    encode8<kMomentTopV, true>(a, ~w, c, e);
     __stcs(reinterpret_cast<uint2*>(vc), make_uint2(pack_bytes(c[0], c[1], c[2], c[3]),
                                                     pack_bytes(c[4], c[5], c[6], c[7])));
     if ((threadIdx.x & 31) == 0) *ve = (uint8_t)e;
