@@ -22,7 +22,8 @@ from __future__ import annotations
 
 import ctypes
 import math
-from operator import attrgetter
+from functools import partial
+from operator import attrgetter, is_
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -41,6 +42,9 @@ _is_contiguous = torch.Tensor.is_contiguous
 _device_index = torch.Tensor.get_device
 _dtype = attrgetter("dtype")
 _shape = attrgetter("shape")
+_numel = torch.Tensor.numel
+_same_size = torch.Tensor.is_same_size
+_is_none = partial(is_, None)
 
 
 def rows_of(t: torch.Tensor) -> Optional[Tuple[int, int]]:
@@ -108,6 +112,9 @@ def _check_tensor(what: str, t) -> None:
 
 
 def _check_cuda(tensors: Sequence[torch.Tensor]) -> torch.device:
+    index = set(map(_device_index, tensors))
+    if len(index) == 1 and index != {-1}:
+        return torch.device("cuda", index.pop())
     devices = {t.device for t in tensors}
     if len(devices) != 1:
         raise ValueError(f"all tensors must be on one device, got {sorted(map(str, devices))}")
@@ -134,10 +141,10 @@ class _on_device:
             torch.cuda.set_device(self.prev)
 
 
-def _norm_partials(lib, entries: np.ndarray, buffer: torch.Tensor, stream: int) -> int:
+def _norm_partials(lib, entries: int, n: int, buffer: torch.Tensor, stream: int) -> int:
     count = ctypes.c_int64(0)
-    _lib.check(lib.gs_grad_norm_partials(entries.ctypes.data, len(entries), buffer.data_ptr(), buffer.numel(),
-                                         ctypes.byref(count), stream), "gradient norm")
+    _lib.check(lib.gs_grad_norm_partials(entries, n, buffer.data_ptr(), buffer.numel(), ctypes.byref(count), stream),
+               "gradient norm")
     return count.value
 
 
@@ -218,7 +225,7 @@ class FusedAdamW:
         e["param_type"] = [TYPES[p.dtype] for p in self._params]
         e["lr_scale"] = [float((lr_scales or {}).get(k, 1.0)) for k in self.names]
         e["decay"] = [self.weight_decay * float((decay_scales or {}).get(k, 1.0)) for k in self.names]
-        self._entries = e
+        self._entries, self._at = e, e.ctypes.data
         dt = torch.float32 if state_bits == 32 else torch.uint8
         self.m = torch.zeros(self.slab_elements, dtype=dt, device=self.device)
         self.v = torch.zeros(self.slab_elements, dtype=dt, device=self.device)
@@ -281,24 +288,34 @@ class FusedAdamW:
         self._ptrs = list(map(_data_ptr, self._params))
         self._entries["param"] = self._ptrs
 
+    def _elements_in(self, entries: np.ndarray) -> bool:
+        return self.slab_elements > 0 if entries is self._entries else bool(entries["n"].any())
+
     def _with_grads(self, entries: np.ndarray, names: Sequence[str], shapes: Sequence[torch.Size],
-                    grads: List[torch.Tensor], what: str = "gradient") -> List[torch.Tensor]:
+                    grads: List[torch.Tensor], what: str = "gradient") -> Tuple[np.ndarray, List[torch.Tensor]]:
         """Fills the entries' second tensor from ``grads`` (checked against
-        ``shapes``); returns the tensors that must outlive the launch."""
-        if not all(isinstance(g, torch.Tensor) for g in grads) or \
-                any(g.layout != torch.strided or g.dtype not in TYPES for g in grads):
+        ``shapes``); returns the entries (a copy where their rows had to change)
+        and the tensors that must outlive the launch."""
+        try:
+            types = list(map(TYPES.__getitem__, map(_dtype, grads)))
+            same = list(map(_shape, grads)) == shapes
+            here = set(map(_device_index, grads)) == {self.device.index}
+            dense = all(map(_is_contiguous, grads))
+            entries["grad"] = list(map(_data_ptr, grads))
+        except (KeyError, AttributeError, TypeError, RuntimeError):
             for name, g in zip(names, grads):
                 _check_tensor(f"{what} of {name!r}", g)
-        if list(map(_shape, grads)) != list(shapes):
+            raise
+        if not same:
             for name, s, g in zip(names, shapes, grads):
                 if g.shape != s:
                     raise ValueError(f"{what} of {name!r} has shape {tuple(g.shape)}, not {tuple(s)}")
-        if set(map(_device_index, grads)) != {self.device.index}:
+        if not here:
             raise ValueError(f"every {what} must be on {self.device}")
-        entries["grad_type"] = [TYPES[d] for d in map(_dtype, grads)]
+        entries["grad_type"] = types
         entries["grad_stride"] = entries["cols"]
-        if not all(map(_is_contiguous, grads)):
-            grads = list(grads)
+        if not dense:
+            entries, grads = entries.copy(), list(grads)
             for k, g in enumerate(grads):
                 if g.is_contiguous():
                     continue
@@ -311,8 +328,8 @@ class FusedAdamW:
                     entries["grad_stride"][k] = rows[1]
                 else:
                     grads[k] = g.contiguous()
-        entries["grad"] = list(map(_data_ptr, grads))
-        return grads
+                    entries["grad"][k] = grads[k].data_ptr()
+        return entries, grads
 
     # ------------------------------------------------------------------ the step
     def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_scale: float = 1.0) -> Optional[torch.Tensor]:
@@ -326,38 +343,39 @@ class FusedAdamW:
         if grads is None:
             found = [p.grad for p in self._params]
         else:
-            if not grads.keys() <= self.offsets.keys():
-                raise ValueError(f"no parameter named {sorted(set(grads) - set(self.names))}")
             found = list(map(grads.get, self.names))
+            if len(grads) != len(found) and not grads.keys() <= self.offsets.keys():
+                raise ValueError(f"no parameter named {sorted(set(grads) - set(self.names))}")
         if not math.isfinite(grad_scale):
             raise ValueError(f"grad_scale must be finite: {grad_scale}")
         lr, lr_device = self._lr_value()
         limit = self._norm_limit()
         if list(map(_data_ptr, self._params)) != self._ptrs:
             self._refresh()
-        names, shapes, params = self.names, self._shapes, self._params
-        if any(g is None for g in found):
+        names, shapes, params, entries = self.names, self._shapes, self._params, self._entries
+        if any(map(_is_none, found)):
+            if grads is not None and not grads.keys() <= self.offsets.keys():
+                raise ValueError(f"no parameter named {sorted(set(grads) - set(self.names))}")
             on = [k for k, g in enumerate(found) if g is not None]
-            entries = self._entries[on]
+            entries = entries[on]
             names, shapes, params, found = ([x[k] for k in on] for x in (names, shapes, params, found))
-        else:
-            entries = self._entries.copy()
         with_norm = self.max_norm is not None or self.skip_nonfinite
         norm = None
         with _on_device(self.device):
             if with_norm:
                 norm = torch.empty((), dtype=torch.float32, device=self.device)
-            if not params or not int(entries["n"].sum()):
+            if not self._elements_in(entries):
                 return norm.zero_() if with_norm else None
-            keep = self._with_grads(entries, names, shapes, found)
+            entries, keep = self._with_grads(entries, names, shapes, found)
+            at = self._at if entries is self._entries else entries.ctypes.data
             stream = _lib.stream_ptr(self.device)
             s = _lib.GsAdamWSettings(lr, self.beta1, self.beta2, self.eps, grad_scale, lr_device, None, 0, limit, None)
             if with_norm:
                 buffer = self._partials_buffer(lib)
-                s.num_partials = _norm_partials(lib, entries, buffer, stream)
+                s.num_partials = _norm_partials(lib, at, len(entries), buffer, stream)
                 s.norm_partials = buffer.data_ptr()
                 s.norm_out = norm.data_ptr()
-            _lib.check(lib.gs_adamw_step(entries.ctypes.data, len(entries), self._state, s, stream), "adamw step")
+            _lib.check(lib.gs_adamw_step(at, len(entries), self._state, s, stream), "adamw step")
             del keep
         torch.autograd.graph.increment_version(params)
         return norm
@@ -410,10 +428,10 @@ class FusedAdamW:
             entries = np.zeros(len(ml), _ENTRY)
             entries["n"], entries["state"] = self._entries["n"], self._entries["state"]
             entries["cols"] = entries["param_stride"] = np.maximum(entries["n"], 1)
-            keep = self._with_grads(entries, self.names, self._shapes, [x.contiguous() for x in ml], "moment m")
-            for a, b in (("param", "grad"), ("param_type", "grad_type")):
-                entries[a] = entries[b]
-            keep = keep + self._with_grads(entries, self.names, self._shapes, [x.contiguous() for x in vl], "moment v")
+            ml, vl = [x.contiguous() for x in ml], [x.contiguous() for x in vl]
+            self._with_grads(entries, self.names, self._shapes, ml, "moment m")
+            entries["param"], entries["param_type"] = entries["grad"], entries["grad_type"]
+            self._with_grads(entries, self.names, self._shapes, vl, "moment v")
             if t is None:
                 t = self.t if self.state_bits == 8 else None
             else:
@@ -427,7 +445,6 @@ class FusedAdamW:
             _lib.check(lib.gs_moments8_quantize(entries.ctypes.data, len(entries), self.m.data_ptr(),
                                                 self.v.data_ptr(), self.m_exp.data_ptr(), self.v_exp.data_ptr(),
                                                 int(t), _lib.stream_ptr(self.device)), "8-bit moments")
-            del keep
 
     def sync_master(self) -> None:
         """Takes the float32 master copies from the parameters again."""
@@ -483,10 +500,6 @@ def _dequantize(m, v, m_exp, v_exp, dtype) -> Tuple[torch.Tensor, torch.Tensor]:
 Tensors = Union[Dict[str, torch.Tensor], Sequence[torch.Tensor]]
 
 
-def _named(tensors: Tensors) -> Dict:
-    return dict(tensors) if isinstance(tensors, dict) else dict(enumerate(tensors))
-
-
 def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = None) -> torch.Tensor:
     """Scales the gradients (name -> tensor, or a sequence) by ``max_norm`` over
     their global norm where that exceeds ``max_norm``, in place, or into the
@@ -497,69 +510,128 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
     max_norm = float(max_norm)
     if not max_norm > 0.0:
         raise ValueError(f"max_norm must be positive: {max_norm}")
-    src = _named(grads)
-    dst = src if out is None else _named(out)
-    if not src:
+    if isinstance(grads, dict):
+        names, gl = list(grads), list(grads.values())
+        if out is not None:
+            if not isinstance(out, dict) or out.keys() != grads.keys():
+                raise ValueError("out must have the gradients' names")
+            ol = list(map(out.__getitem__, names))
+    else:
+        names, gl = range(len(grads)), list(grads)
+        if out is not None:
+            ol = list(out)
+            if len(ol) != len(gl):
+                raise ValueError(f"{len(ol)} tensors in out for {len(gl)} gradients")
+    if not gl:
         raise ValueError("no gradients")
-    if src.keys() != dst.keys():
-        raise ValueError("out must have the gradients' names")
-    gl, ol = list(src.values()), [dst[k] for k in src]
-    entries = np.zeros(len(gl), _ENTRY)
-    for k, (name, g, o) in enumerate(zip(src, gl, ol)):
-        _check_tensor(f"gradient {name!r}", g)
-        if o is not g:
+    if out is None:
+        ol = gl
+    try:
+        entries = _clip_entries(gl, ol)
+    except (KeyError, AttributeError, TypeError, RuntimeError):
+        for name, g, o in zip(names, gl, ol):
+            _check_tensor(f"gradient {name!r}", g)
             _check_tensor(f"out {name!r}", o)
-            if o.shape != g.shape:
-                raise ValueError(f"out {name!r} has shape {tuple(o.shape)}, not {tuple(g.shape)}")
-    g_rows = list(map(rows_of, gl))
-    o_rows = g_rows if out is None else list(map(rows_of, ol))
-    for k, name in enumerate(src):
-        if o_rows[k] is None:
-            raise ValueError(f"{'gradient' if out is None else 'out'} {name!r}: strides {tuple(ol[k].stride())} of "
-                             f"shape {tuple(ol[k].shape)} are neither dense nor rows at one distance")
-    both = overlapping(ol, o_rows)
-    if both is not None:
-        raise ValueError("written tensors share memory")
-    if out is not None:
-        _check_apart(gl, g_rows, ol, o_rows)
+        raise
+    if entries is None:
+        entries, gl = _clip_entries_strided(names, gl, ol)
     device = _check_cuda(gl + ol)
     lib = _lib.lib()
     with _on_device(device):
-        for k in range(len(gl)):
-            dense = g_rows[k] is not None and g_rows[k][0] == g_rows[k][1]
-            if g_rows[k] is None or not (dense or o_rows[k][0] in (o_rows[k][1], g_rows[k][0])):
-                gl[k] = gl[k].contiguous()
-                g_rows[k] = rows_of(gl[k])
-                dense = True
-            cols = o_rows[k][0] if dense else g_rows[k][0]
-            entries[k] = (ol[k].data_ptr(), gl[k].data_ptr(), gl[k].numel(), 0, cols,
-                          cols if o_rows[k][0] == o_rows[k][1] else o_rows[k][1], cols if dense else g_rows[k][1],
-                          TYPES[ol[k].dtype], TYPES[gl[k].dtype], 1.0, 0.0)
         norm = torch.empty((), dtype=torch.float32, device=device)
-        if not int(entries["n"].sum()):
+        if not entries["n"].any():
             return norm.zero_()
-        stream = _lib.stream_ptr(device)
-        partials = torch.empty(lib.gs_grad_norm_max_partials(len(entries)), dtype=torch.float64, device=device)
-        count = _norm_partials(lib, entries, partials, stream)
-        _lib.check(lib.gs_clip_gradients(entries.ctypes.data, len(entries), partials.data_ptr(), count, max_norm,
-                                         norm.data_ptr(), stream), "clip gradients")
+        at, n, stream = entries.ctypes.data, len(entries), _lib.stream_ptr(device)
+        partials = torch.empty(lib.gs_grad_norm_max_partials(n), dtype=torch.float64, device=device)
+        count = _norm_partials(lib, at, n, partials, stream)
+        _lib.check(lib.gs_clip_gradients(at, n, partials.data_ptr(), count, max_norm, norm.data_ptr(), stream),
+                   "clip gradients")
     torch.autograd.graph.increment_version(ol)
     return norm
 
 
-def _check_apart(gl, g_rows, ol, o_rows) -> None:
+def _codes(tensors: List[torch.Tensor]):
+    """Type codes of the tensors: one number where they are all of one type."""
+    types = list(map(_dtype, tensors))
+    return TYPES[types[0]] if types.count(types[0]) == len(types) else np.array([TYPES[t] for t in types])
+
+
+def _clip_entries(gl: List[torch.Tensor], ol: List[torch.Tensor]) -> Optional[np.ndarray]:
+    """The entries where every tensor is dense and none shares memory that
+    another one writes; None where that takes a closer look."""
+    if not all(map(_is_contiguous, gl)):
+        return None
+    n = len(gl)
+    words = np.zeros((n, _ENTRY.itemsize // 8), np.int64)  # the entries' fields, the two types sharing a word
+    size = words[:, 2]
+    size[:] = list(map(_numel, gl))
+    words[:, 4:7] = np.maximum(size, 1)[:, None]
+    g_type = o_type = _codes(gl)
+    g_ptr = words[:, 1]
+    g_ptr[:] = list(map(_data_ptr, gl))
+    o_ptr = words[:, 0]
+    if ol is gl:
+        o_ptr[:] = g_ptr
+    else:
+        if not (all(map(_is_contiguous, ol)) and all(map(_same_size, gl, ol))):
+            return None
+        o_type = _codes(ol)
+        o_ptr[:] = list(map(_data_ptr, ol))
+    words[:, 7] = o_type + g_type * (1 << 32)
+    o_end = o_ptr + size * (4 - 2 * (o_type != _lib.GS_F32))
+    order = o_ptr.argsort()
+    starts, ends = o_ptr[order], o_end[order]
+    if n > 1 and (ends[:-1] > starts[1:]).any():
+        return None
+    if ol is not gl:
+        # a gradient may lie in its own output's memory, or in none: the last output that starts below its end
+        g_end = g_ptr + size * (4 - 2 * (g_type != _lib.GS_F32))
+        last = starts.searchsorted(g_end) - 1
+        shared = (ends[last] > g_ptr) & (last >= 0)
+        if shared.any() and (shared & ((g_ptr != o_ptr) | (g_type != o_type))).any():
+            return None
+    return words.view(_ENTRY).reshape(n)
+
+
+def _clip_entries_strided(names, gl: List[torch.Tensor], ol: List[torch.Tensor]):
+    """The entries of any tensors, with the refusals; and the gradients, dense
+    copies in the place of those that are not rows."""
+    in_place = ol is gl
+    for name, g, o in zip(names, gl, ol):
+        _check_tensor(f"gradient {name!r}", g)
+        _check_tensor(f"out {name!r}", o)
+        if o.shape != g.shape:
+            raise ValueError(f"out {name!r} has shape {tuple(o.shape)}, not {tuple(g.shape)}")
+    g_rows, o_rows = list(map(rows_of, gl)), list(map(rows_of, ol))
+    for name, o, rows in zip(names, ol, o_rows):
+        if rows is None:
+            raise ValueError(f"{'gradient' if in_place else 'out'} {name!r}: strides {tuple(o.stride())} of shape "
+                             f"{tuple(o.shape)} are neither dense nor rows at one distance")
+    if overlapping(ol, o_rows) is not None:
+        raise ValueError("written tensors share memory")
+    if not in_place:
+        _check_apart(gl, ol, o_rows)
+    gl = list(gl)
+    entries = np.zeros(len(gl), _ENTRY)
+    for k, (g, o) in enumerate(zip(gl, ol)):
+        (o_cols, o_stride), rows = o_rows[k], g_rows[k]
+        if rows is None or not (rows[0] == rows[1] or o_cols in (o_stride, rows[0])):
+            g = gl[k] = g.contiguous()
+            rows = rows_of(g)
+        g_dense, o_dense = rows[0] == rows[1], o_cols == o_stride
+        cols = o_cols if g_dense else rows[0]
+        entries[k] = (o.data_ptr(), g.data_ptr(), g.numel(), 0, cols, cols if o_dense else o_stride,
+                      cols if g_dense else rows[1], TYPES[o.dtype], TYPES[g.dtype], 1.0, 0.0)
+    return entries, gl
+
+
+def _check_apart(gl: List[torch.Tensor], ol: List[torch.Tensor], o_rows) -> None:
     """A written tensor may be its own gradient's memory, but no other's."""
     spans = sorted(_span(o, r) for o, r in zip(ol, o_rows) if o.numel())
-    starts, ends = [s for s, _ in spans], [e for _, e in spans]
-    if not spans:
-        return
-    for k, g in enumerate(gl):
-        if not g.numel() or (g.data_ptr() == ol[k].data_ptr() and g.dtype == ol[k].dtype and
-                             g.stride() == ol[k].stride()):
+    for g, o in zip(gl, ol):
+        if not g.numel() or (g.data_ptr() == o.data_ptr() and g.dtype == o.dtype and g.stride() == o.stride()):
             continue
         lo = g.data_ptr()
         hi = lo + (sum((d - 1) * s for d, s in zip(g.shape, g.stride())) + 1) * g.element_size()
-        at = int(np.searchsorted(starts, hi)) - 1
-        # spans of strided outputs may nest, so every span that starts before ``hi`` counts
-        if at >= 0 and max(ends[:at + 1]) > lo:
+        if any(a < hi and b > lo for a, b in spans):
             raise ValueError("a written tensor shares memory with another gradient")

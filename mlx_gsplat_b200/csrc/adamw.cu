@@ -17,7 +17,16 @@
 
 namespace gs {
 
-constexpr int kAdamWBlocksPerSm = 3;
+// Resident blocks per SM and the largest group of chunks a block takes at a time.
+// 32-bit moments: the step is a copy of seven streams, and two blocks of 256
+// threads already have enough in flight; three are slower, since more reads and
+// writes at once disturb one another in DRAM (59M parameters: 256 us with two, 297
+// with three), and single chunks keep the blocks closest together.  8-bit moments:
+// nearly as much arithmetic as memory time, so the registers' most, three; groups
+// as large as the exponents' (moments8.cuh) and no larger.
+constexpr int kBlocks32 = 2, kGroup32 = 1;
+constexpr int kBlocks8 = 3, kGroup8 = 16;
+constexpr int kBlocksQuantize = 4;
 
 struct AdamWArgs {
     void *m, *v;
@@ -99,128 +108,232 @@ __device__ __forceinline__ float param_update(float p, float m, float v, float i
     return fmaf(-step, m * inv, p * keep);
 }
 
+// What a tensor's elements share in the step.
+struct AdamWTensor {
+    float step, keep, gscale, inv_sqrt_bc2;
+    uint32_t step_word;
+};
+
+__device__ __forceinline__ void update8(float (&p)[8], const float (&g)[8], float (&m)[8], float (&v)[8],
+                                        const AdamWTensor& t, const AdamWArgs& a) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        moments_update(__fmul_rn(g[k], t.gscale), m[k], v[k], a);
+        p[k] = param_update(p[k], m[k], v[k], t.inv_sqrt_bc2, t.step, t.keep, a.eps);
+    }
+}
+
+// ``count`` whole chunks of a tensor from element i on, all accesses 16 bytes wide.
+// kWideP: float32 parameters (or masters: kMaster, with 16-bit parameters written
+// from them); kWideG: float32 gradients.
+template <int kBits, bool kWideP, bool kWideG, bool kMaster>
+__device__ __forceinline__ void adamw_chunks(const TensorEntry& e, const AdamWArgs& a, const AdamWTensor& t, int64_t i,
+                                             int count, BlockExponents& x) {
+    constexpr int kState = kBits / 8;
+    const int64_t s = e.state + i;
+    char* m_at = static_cast<char*>(a.m) + s * kState;
+    char* v_at = static_cast<char*>(a.v) + s * kState;
+    const char* g_at = static_cast<const char*>(e.grad) + i * (kWideG ? 4 : 2);
+    char* p_at = kMaster ? reinterpret_cast<char*>(a.master + s) : static_cast<char*>(e.param) + i * (kWideP ? 4 : 2);
+    char* p16_at = static_cast<char*>(e.param) + i * 2;
+    const int p_type = e.param_type, g_type = e.grad_type;
+    uint32_t index = (uint32_t)i;
+    for (int j = 0; j < count; ++j) {
+        Raw8 rm, rv;
+        uint2 cm, cv;
+        if (kBits == 32) {
+            rm = load_raw8<true>(m_at);
+            rv = load_raw8<true>(v_at);
+        } else {
+            cm = __ldcs(reinterpret_cast<const uint2*>(m_at));
+            cv = __ldcs(reinterpret_cast<const uint2*>(v_at));
+        }
+        const Raw8 rg = load_raw8<kWideG>(g_at);
+        const Raw8 rp = load_raw8<kWideP || kMaster>(p_at);
+        float p[8], g[8], m[8], v[8];
+        unpack8<kWideG>(rg, g_type, g);
+        if (kBits == 32) {
+            unpack8<true>(rm, GS_F32, m);
+            unpack8<true>(rv, GS_F32, v);
+        } else {
+            decode_m8(cm, __shfl_sync(kFull, x.m, j), m);
+            decode_v8(cv, __shfl_sync(kFull, x.v, j), v);
+        }
+        unpack8<kWideP || kMaster>(rp, p_type, p);
+        update8(p, g, m, v, t, a);
+        store_vec8<kWideP || kMaster>(p_at, p_type, p);
+        if (kMaster) store_vec8<false>(p16_at, p_type, p);
+        if (kBits == 32) {
+            store_vec8<true, true>(m_at, GS_F32, m);
+            store_vec8<true, true>(v_at, GS_F32, v);
+        } else {
+            uint32_t em, ev;
+            store_moments8<false>(m, v, index, t.step_word, reinterpret_cast<uint8_t*>(m_at),
+                                  reinterpret_cast<uint8_t*>(v_at), em, ev);
+            x.set(j, em, ev);
+        }
+        m_at += kChunk * kState;
+        v_at += kChunk * kState;
+        g_at += kChunk * (kWideG ? 4 : 2);
+        p_at += kChunk * (kWideP || kMaster ? 4 : 2);
+        p16_at += kChunk * 2;
+        index += kChunk;
+    }
+}
+
+// One warp's block of a chunk, where the tensor's end, strides or alignment ask for
+// single accesses.  ``em``, ``ev``: the block's exponents; returns the new ones, v's
+// in the second byte.
+template <int kBits>
+__device__ __forceinline__ uint32_t adamw_ragged(const TensorEntry& e, const AdamWArgs& a, AdamWTensor t, int64_t i,
+                                              uint32_t em, uint32_t ev) {
+    const int64_t s = e.state + i;
+    const bool masters = a.master != nullptr && e.param_type != GS_F32;
+    float p[8], g[8], m[8], v[8];
+    load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, e.grad_vec, g);
+    if (masters)
+        unpack8(load_raw8(a.master, s, GS_F32), GS_F32, p);
+    else
+        load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, p);
+    if (kBits == 32) {
+        unpack8(load_raw8(a.m, s, GS_F32), GS_F32, m);
+        unpack8(load_raw8(a.v, s, GS_F32), GS_F32, v);
+    } else {
+        decode_m8(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + s), em, m);
+        decode_v8(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + s), ev, v);
+    }
+    update8(p, g, m, v, t, a);
+    if (masters) store_vec8(a.master, s, GS_F32, p);
+    store_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, p);
+    if (kBits == 32) {
+        store_vec8(a.m, s, GS_F32, m);
+        store_vec8(a.v, s, GS_F32, v);
+        return 0;
+    }
+    store_moments8<false>(m, v, (uint32_t)i, t.step_word, static_cast<uint8_t*>(a.m) + s,
+                          static_cast<uint8_t*>(a.v) + s, em, ev);
+    return em | ev << 8;
+}
+
 template <int kBits, int kCap>
-__global__ void __launch_bounds__(kMultiThreads, kAdamWBlocksPerSm) adamw_kernel(
+__global__ void __launch_bounds__(kMultiThreads, kBits == 32 ? kBlocks32 : kBlocks8) adamw_kernel(
     const __grid_constant__ TensorTable<kCap> tab, const __grid_constant__ AdamWArgs a) {
     __shared__ AdamWShared sh;
     pdl_wait();
-    int c, end;
-    block_share(tab, c, end);
-    int ti = find_tensor(tab, c);
-    float step = 0.0f, keep = 0.0f;
-    // the grid has at most one block per chunk, so every block has a first chunk
-    for (int seen = -1; c < end; ++c) {
-        while (c >= tab.first[ti + 1]) ++ti;
-        const TensorEntry& e = tab.e[ti];
-        const int64_t i = (int64_t)(c - tab.first[ti]) * kChunk + threadIdx.x * kPerThread;
-        const int64_t s = e.state + i;
-        // the state has whole blocks of 256, so a warp is inside or outside as one
-        const bool inside = i - (threadIdx.x & 31) * kPerThread < e.n;
-        const bool whole = i + kPerThread <= e.n;
+    Segments<kCap> seg(tab);
+    int chunks;
+    int64_t i;
+    bool more = seg.next(chunks, i);  // every block has a chunk
+    adamw_prologue(a, sh);
+    if (sh.skip) return;
+    AdamWTensor t;
+    t.gscale = sh.gscale;
+    t.inv_sqrt_bc2 = sh.inv_sqrt_bc2;
+    t.step_word = sh.step_word;
+    for (; more; more = seg.next(chunks, i)) {
+        const TensorEntry& e = tab.e[seg.tensor];
+        const double lr = sh.lr * e.lr_scale;
+        t.step = (float)(lr * sh.inv_bc1);
+        t.keep = (float)(1.0 - lr * e.decay);
+        i += threadIdx.x * kPerThread;
+        int mine, whole;
+        warp_chunks(e.n, i, chunks, mine, whole);
+        const int64_t block = (e.state + i) / GS_MOMENT_BLOCK;
+        BlockExponents x;
+        if (kBits == 8) x.load(a.m_exp, a.v_exp, block, kChunk / GS_MOMENT_BLOCK, mine);
         const bool masters = a.master != nullptr && e.param_type != GS_F32;
-        const bool vg = whole && e.grad_vec, vp = whole && e.param_vec;
-        Raw8 rp, rg, rm, rv;
-        uint2 cm, cv;
-        uint32_t em = 0, ev = 0;
-        if (inside) {
-            if (kBits == 32) {
-                rm = load_raw8(a.m, s, GS_F32);
-                rv = load_raw8(a.v, s, GS_F32);
+        int done = 0;
+        if (e.param_vec && e.grad_vec) {
+            done = whole;
+            const bool wide_g = e.grad_type == GS_F32;
+            if (e.param_type == GS_F32) {
+                if (wide_g)
+                    adamw_chunks<kBits, true, true, false>(e, a, t, i, done, x);
+                else
+                    adamw_chunks<kBits, true, false, false>(e, a, t, i, done, x);
+            } else if (masters) {
+                if (wide_g)
+                    adamw_chunks<kBits, false, true, true>(e, a, t, i, done, x);
+                else
+                    adamw_chunks<kBits, false, false, true>(e, a, t, i, done, x);
             } else {
-                cm = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + s));
-                cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + s));
-                em = a.m_exp[s / GS_MOMENT_BLOCK];
-                ev = a.v_exp[s / GS_MOMENT_BLOCK];
+                if (wide_g)
+                    adamw_chunks<kBits, false, true, false>(e, a, t, i, done, x);
+                else
+                    adamw_chunks<kBits, false, false, false>(e, a, t, i, done, x);
             }
-            if (vg) rg = load_raw8(e.grad, i, e.grad_type);
-            if (masters)
-                rp = load_raw8(a.master, s, GS_F32);
-            else if (vp)
-                rp = load_raw8(e.param, i, e.param_type);
         }
-        if (ti != seen) {
-            // the first chunk's loads are on their way while the block forms what the step shares
-            if (seen < 0) {
-                adamw_prologue(a, sh);
-                if (sh.skip) return;
-            }
-            const double lr = sh.lr * e.lr_scale;
-            step = (float)(lr * sh.inv_bc1);
-            keep = (float)(1.0 - lr * e.decay);
-            seen = ti;
+        for (; done < mine; ++done) {
+            const uint32_t em = kBits == 8 ? __shfl_sync(kFull, x.m, done) : 0;
+            const uint32_t ev = kBits == 8 ? __shfl_sync(kFull, x.v, done) : 0;
+            const uint32_t both = adamw_ragged<kBits>(e, a, t, i + (int64_t)done * kChunk, em, ev);
+            if (kBits == 8) x.set(done, both & 255u, both >> 8);
         }
-        if (!inside) continue;
-        float p[8], g[8], m[8], v[8];
-        if (vg)
-            unpack8(rg, e.grad_type, g);
-        else
-            load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, g);
-        if (kBits == 32) {
-            unpack8(rm, GS_F32, m);
-            unpack8(rv, GS_F32, v);
-        } else {
-            decode_m8(cm, em, m);
-            decode_v8(cv, ev, v);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) moments_update(__fmul_rn(g[k], sh.gscale), m[k], v[k], a);
-        if (masters)
-            unpack8(rp, GS_F32, p);
-        else if (vp)
-            unpack8(rp, e.param_type, p);
-        else
-            load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, p);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) p[k] = param_update(p[k], m[k], v[k], sh.inv_sqrt_bc2, step, keep, a.eps);
-        if (masters) store_vec8(a.master, s, GS_F32, p);
-        if (vp)
-            store_vec8(e.param, i, e.param_type, p);
-        else
-            store_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, p);
-        if (kBits == 32) {
-            store_vec8(a.m, s, GS_F32, m);
-            store_vec8(a.v, s, GS_F32, v);
-        } else {
-            store_moments8<false>(m, v, (uint32_t)i, sh.step_word, static_cast<uint8_t*>(a.m) + s,
-                                  static_cast<uint8_t*>(a.v) + s, a.m_exp + s / GS_MOMENT_BLOCK,
-                                  a.v_exp + s / GS_MOMENT_BLOCK);
-        }
+        if (kBits == 8) x.store(a.m_exp, a.v_exp, block, kChunk / GS_MOMENT_BLOCK, mine);
     }
+}
+
+// Whole chunks of float32 moments.
+__device__ __forceinline__ void quantize_chunks(const TensorEntry& e, uint8_t* mc, uint8_t* vc, int64_t i, int count,
+                                                uint32_t step_word, BlockExponents& x) {
+    const float* m_at = static_cast<const float*>(e.param) + i;
+    const float* v_at = static_cast<const float*>(e.grad) + i;
+    mc += e.state + i;
+    vc += e.state + i;
+    uint32_t index = (uint32_t)i;
+    for (int j = 0; j < count; ++j) {
+        const Raw8 rm = load_raw8<true>(m_at), rv = load_raw8<true>(v_at);
+        float m[8], v[8];
+        unpack8<true>(rm, GS_F32, m);
+        unpack8<true>(rv, GS_F32, v);
+        uint32_t em, ev;
+        store_moments8<true>(m, v, index, step_word, mc, vc, em, ev);
+        x.set(j, em, ev);
+        m_at += kChunk;
+        v_at += kChunk;
+        mc += kChunk;
+        vc += kChunk;
+        index += kChunk;
+    }
+}
+
+__device__ __forceinline__ uint32_t quantize_ragged(const TensorEntry& e, uint8_t* mc, uint8_t* vc, int64_t i,
+                                                 uint32_t step_word) {
+    float m[8], v[8];
+    load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, m);
+    load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, e.grad_vec, v);
+    uint32_t em, ev;
+    store_moments8<true>(m, v, (uint32_t)i, step_word, mc + e.state + i, vc + e.state + i, em, ev);
+    return em | ev << 8;
 }
 
 // m (the entries' param) and v (their grad) of any type -> the 8-bit form, with
 // step t's offsets.
 template <int kCap>
-__global__ void __launch_bounds__(kMultiThreads) moments8_quantize_kernel(const __grid_constant__ TensorTable<kCap> tab,
-                                                                          uint8_t* mc, uint8_t* vc, uint8_t* me,
-                                                                          uint8_t* ve, uint32_t step_word) {
+__global__ void __launch_bounds__(kMultiThreads, kBlocksQuantize) moments8_quantize_kernel(
+    const __grid_constant__ TensorTable<kCap> tab, uint8_t* mc, uint8_t* vc, uint8_t* me, uint8_t* ve,
+    uint32_t step_word) {
     pdl_wait();
-    int c, end;
-    block_share(tab, c, end);
-    if (c >= end) return;
-    int ti = find_tensor(tab, c);
-    for (; c < end; ++c) {
-        while (c >= tab.first[ti + 1]) ++ti;
-        const TensorEntry& e = tab.e[ti];
-        const int64_t i = (int64_t)(c - tab.first[ti]) * kChunk + threadIdx.x * kPerThread;
-        const int64_t s = e.state + i;
-        if (i - (threadIdx.x & 31) * kPerThread >= e.n) continue;
-        const bool whole = i + kPerThread <= e.n;
-        float m[8], v[8];
-        Raw8 rm, rv;
-        const bool vm = whole && e.param_vec, vv = whole && e.grad_vec;
-        if (vm) rm = load_raw8(e.param, i, e.param_type);
-        if (vv) rv = load_raw8(e.grad, i, e.grad_type);
-        if (vm)
-            unpack8(rm, e.param_type, m);
-        else
-            load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, m);
-        if (vv)
-            unpack8(rv, e.grad_type, v);
-        else
-            load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, v);
-        store_moments8<true>(m, v, (uint32_t)i, step_word, mc + s, vc + s, me + s / GS_MOMENT_BLOCK,
-                       ve + s / GS_MOMENT_BLOCK);
+    Segments<kCap> seg(tab);
+    int chunks;
+    int64_t i;
+    while (seg.next(chunks, i)) {
+        const TensorEntry& e = tab.e[seg.tensor];
+        i += threadIdx.x * kPerThread;
+        int mine, whole;
+        warp_chunks(e.n, i, chunks, mine, whole);
+        const int64_t block = (e.state + i) / GS_MOMENT_BLOCK;
+        BlockExponents x;
+        int done = 0;
+        if (e.param_vec && e.grad_vec && e.param_type == GS_F32 && e.grad_type == GS_F32) {
+            quantize_chunks(e, mc, vc, i, whole, step_word, x);
+            done = whole;
+        }
+        for (; done < mine; ++done) {
+            const uint32_t both = quantize_ragged(e, mc, vc, i + (int64_t)done * kChunk, step_word);
+            x.set(done, both & 255u, both >> 8);
+        }
+        x.store(me, ve, block, kChunk / GS_MOMENT_BLOCK, mine);
     }
 }
 
@@ -254,7 +367,8 @@ static int adamw_launches(const gs_tensor* t, int64_t count, int bits, AdamWArgs
         a.advance = left == 0;
         void* args[] = {&tab, &a};
         const void* k = bits == 32 ? (const void*)adamw_kernel<32, kCap> : (const void*)adamw_kernel<8, kCap>;
-        GS_TRY(launch_table("adamw_kernel", k, table_grid(tab, kAdamWBlocksPerSm), stream, args));
+        const int grid = bits == 32 ? table_grid(tab, kBlocks32, kGroup32) : table_grid(tab, kBlocks8, kGroup8);
+        GS_TRY(launch_table("adamw_kernel", k, grid, stream, args));
     }
     return GS_OK;
 }
@@ -269,7 +383,7 @@ static int quantize_launches(const gs_tensor* t, int64_t count, uint8_t* m, uint
         left -= tab.count;
         void* args[] = {&tab, &m, &v, &me, &ve, &step_word};
         GS_TRY(launch_table("moments8_quantize_kernel", (const void*)moments8_quantize_kernel<kCap>,
-                            table_grid(tab, 4), stream, args));
+                            table_grid(tab, kBlocksQuantize, kGroup8), stream, args));
     }
     return GS_OK;
 }

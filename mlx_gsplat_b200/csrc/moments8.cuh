@@ -20,9 +20,11 @@
 //
 // A magnitude is rounded in its float32 bits: bits + u (20 bits) cut to the upper 3
 // mantissa bits is floor(x / step + u) * step for every x of a whole binade, and
-// its carry moves to the next binade by itself.  Below field 1 the step is fixed:
-// x is scaled so that a step is 2^20, cut by adding 2^23 with rounding toward
-// zero, and offset in integers.
+// its carry moves to the next binade by itself.  Below L, the smallest value with
+// field 1, the step is fixed: L + x, added with rounding toward zero, holds x in
+// units of 2^-20 of that step, and its bits less 2^23 continue those of the values
+// above.  They are the larger of the two forms exactly where x < L (the bits of a
+// float32 are a concave function of it), so one maximum selects, without a branch.
 #pragma once
 
 #include "common.cuh"
@@ -95,57 +97,85 @@ __device__ __forceinline__ uint32_t pack_tops(uint32_t a, uint32_t b, uint32_t c
 template <int kTop, bool kPositive>
 __device__ __forceinline__ void encode8(const uint32_t (&a)[8], uint32_t w, uint32_t (&code)[8], uint32_t& e) {
     constexpr uint32_t kNext = kPositive ? 0u - kDitherElement : kDitherElement;
-    uint32_t most = 0, least = 0xffffffffu;
+    uint32_t most = a[0];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        code[k] = a[k] + ((w + (uint32_t)k * kNext) >> 12);
-        most = max(most, code[k]);
-        least = min(least, a[k] - 1u);  // a zero is no small value: it wraps to the largest
+    for (int k = 1; k < 8; ++k) most = max(most, a[k]);
+    most = __reduce_max_sync(kFull, most);
+    if ((most >> 20 & 7u) == 7u) {
+        // only from the last eighth of a binade can a rounding carry into the next one
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = max(most, a[k] + ((w + (uint32_t)k * kNext) >> 12));
+        most = __reduce_max_sync(kFull, most);
     }
-    e = min(max(__reduce_max_sync(kFull, most) >> 23, kMomentMinExp), 255u);
-    const uint32_t low = (e - (kTop - 1)) << 23;  // smallest magnitude with exponent field 1
+    e = min(max(most >> 23, kMomentMinExp), 255u);
+    const uint32_t low = (e - (kTop - 1)) << 23;  // L, the smallest magnitude with exponent field 1
     const int base = (int)(e - kTop) << 3;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) code[k] = (uint32_t)max((int)(code[k] >> 20) - base, 0);
-    // Values below field 1 are few (2^-14 of the block's largest for m, 2^-30 for v), so warps without any skip them.
-    if (__any_sync(kFull, least < low - 1u)) {
-        // step of field 0 -> 2^20: the factor is 2^(127 + 3 + 20 - (e - (T - 1)))
-        const float f = __uint_as_float((277u + (kTop - 1) - e) << 23);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (a[k] < low) {
-                const float y = __fadd_rz(__fmul_rn(__uint_as_float(a[k]), f), 8388608.0f);
-                code[k] = (__float_as_uint(y) - 0x4B000000u + ((w + (uint32_t)k * kNext) >> 12)) >> 20;
-                if (kPositive && code[k] == 0 && a[k] != 0) code[k] = 1;
-            }
-        }
+    for (int k = 0; k < 8; ++k) {
+        const float fixed = __fadd_rz(__uint_as_float(a[k]), __uint_as_float(low));
+        const uint32_t z = (uint32_t)max((int)a[k], (int)(__float_as_uint(fixed) - (1u << 23)));
+        const int c = (int)((z + ((w + (uint32_t)k * kNext) >> 12)) >> 20) - base;
+        code[k] = (uint32_t)(kPositive ? max(c, (int)min(a[k], 1u)) : c);
     }
 }
 
-// A lane's eight values of both moments -> codes, stored with the block's
+// A lane's eight values of both moments -> codes, stored, and the block's
 // exponents.  All 32 lanes of the warp that holds the block take part.  kAnyV: v
 // may come with a sign (a caller's; the step's own has none).
 template <bool kAnyV>
 __device__ __forceinline__ void store_moments8(const float (&m)[8], const float (&v)[8], uint32_t i, uint32_t step_word,
-                                               uint8_t* mc, uint8_t* vc, uint8_t* me, uint8_t* ve) {
+                                               uint8_t* mc, uint8_t* vc, uint32_t& me, uint32_t& ve) {
     const uint32_t w = i * kDitherElement + step_word;
-    uint32_t a[8], c[8], e;
+    uint32_t a[8], c[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) a[k] = __float_as_uint(m[k]) & 0x7fffffffu;
-    encode8<kMomentTopM, false>(a, w, c, e);
+    encode8<kMomentTopM, false>(a, w, c, me);
     uint2 out = make_uint2(pack_bytes(c[0], c[1], c[2], c[3]), pack_bytes(c[4], c[5], c[6], c[7]));
 #pragma unroll
     for (int k = 0; k < 8; ++k) a[k] = __float_as_uint(m[k]);
     out.x = (out.x & 0x7f7f7f7fu) | (pack_tops(a[0], a[1], a[2], a[3]) & 0x80808080u);
     out.y = (out.y & 0x7f7f7f7fu) | (pack_tops(a[4], a[5], a[6], a[7]) & 0x80808080u);
     __stcs(reinterpret_cast<uint2*>(mc), out);
-    if ((threadIdx.x & 31) == 0) *me = (uint8_t)e;
 #pragma unroll
     for (int k = 0; k < 8; ++k) a[k] = __float_as_uint(v[k]) & (kAnyV ? 0x7fffffffu : 0xffffffffu);
-    encode8<kMomentTopV, true>(a, ~w, c, e);
+    encode8<kMomentTopV, true>(a, ~w, c, ve);
     __stcs(reinterpret_cast<uint2*>(vc), make_uint2(pack_bytes(c[0], c[1], c[2], c[3]),
                                                     pack_bytes(c[4], c[5], c[6], c[7])));
-    if ((threadIdx.x & 31) == 0) *ve = (uint8_t)e;
 }
+
+// The exponent bytes of the blocks that a warp meets in up to 32 successive chunks
+// of a tensor, one block a chunk: lane l holds those of chunk l.  They are read
+// together before the first chunk and written together after the last.  One byte
+// read and written per block and chunk, between those of the other warps in the
+// same 32-byte sector, made every read wait for its neighbours' writes: 245 us
+// instead of 180 us for a step over 59M parameters.
+constexpr int kSegment = 32;  // the largest group of chunks a block may take
+
+struct BlockExponents {
+    uint32_t m, v;
+    // ``first``: the warp's block in the segment's first chunk; ``stride``: blocks from chunk to chunk;
+    // ``count``: chunks in which the warp has a block
+    __device__ __forceinline__ void load(const uint8_t* me, const uint8_t* ve, int64_t first, int stride, int count) {
+        const int lane = threadIdx.x & 31;
+        m = v = 0;
+        if (lane < count) {
+            m = me[first + lane * stride];
+            v = ve[first + lane * stride];
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* me, uint8_t* ve, int64_t first, int stride, int count) const {
+        const int lane = threadIdx.x & 31;
+        if (lane < count) {
+            me[first + lane * stride] = (uint8_t)m;
+            ve[first + lane * stride] = (uint8_t)v;
+        }
+    }
+    __device__ __forceinline__ void set(int chunk, uint32_t em, uint32_t ev) {
+        if ((threadIdx.x & 31) == chunk) {
+            m = em;
+            v = ev;
+        }
+    }
+};
 
 }  // namespace gs

@@ -5,8 +5,8 @@
 // The table travels in the kernel's parameters (at most 32,764 bytes), so a call
 // needs no copy to the device, owns no memory and can be captured into a graph.
 // Elements are handled in chunks of kChunk; the chunks of all tensors form one
-// sequence (``first`` holds each tensor's place in it) and every block takes an
-// equal, contiguous share, so one large tensor and many tiny ones balance alike.
+// sequence (``first`` holds each tensor's place in it) of which every block takes
+// equal shares, so one large tensor and many tiny ones balance alike.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -27,7 +27,7 @@ struct TensorEntry {
     int64_t cols, param_stride, grad_stride;
     double lr_scale, decay;
     int16_t param_type, grad_type;
-    int8_t param_vec, grad_vec;  // dense and aligned for 16-byte accesses
+    int8_t param_vec, grad_vec;  // dense and aligned for accesses to eight elements
 };
 
 template <int kCap>
@@ -35,6 +35,7 @@ struct TensorTable {
     TensorEntry e[kCap];
     int32_t first[kCap + 1];
     int32_t count;
+    int32_t group, groups;  // chunks that a block takes at a time, and how many such groups there are
 };
 
 // Table sizes: a small one for the handful of tensors of a scene (a 2 KB
@@ -44,47 +45,60 @@ constexpr int kSmallTable = 24;
 constexpr int kLargeTable = 368;
 
 // ---------------------------------------------------------------- device side
+// Eight consecutive elements as they lie in memory: 32 bytes of float32 or 16.
+// (One 256-bit access for float32 instead of two of 128 measured the same in the
+// steps and slower in the moments' quantization, 120 us against 104 for 59M.)
 struct Raw8 {
     uint4 a, b;
 };
 
-__device__ __forceinline__ Raw8 load_raw8(const void* base, int64_t i, int type) {
+// kStream: not expected to be read again soon (evicted first from L2).
+template <bool kStream>
+__device__ __forceinline__ uint4 load16(const uint4* p) {
+    return kStream ? __ldcs(p) : *p;
+}
+
+// kWide: float32; else the two 16-bit types.
+template <bool kWide, bool kStream = true>
+__device__ __forceinline__ Raw8 load_raw8(const void* p) {
     Raw8 r;
-    if (type == GS_F32) {
-        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + i);
-        r.a = __ldcs(p);
-        r.b = __ldcs(p + 1);
-    } else {
-        r.a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i));
-        r.b = make_uint4(0, 0, 0, 0);
-    }
+    r.a = load16<kStream>(static_cast<const uint4*>(p));
+    r.b = kWide ? load16<kStream>(static_cast<const uint4*>(p) + 1) : make_uint4(0, 0, 0, 0);
     return r;
 }
 
-__device__ __forceinline__ float2 unpack2(uint32_t w, int type) {
-    if (type == GS_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+__device__ __forceinline__ Raw8 load_raw8(const void* base, int64_t i, int type) {
+    return type == GS_F32 ? load_raw8<true>(static_cast<const float*>(base) + i)
+                          : load_raw8<false>(static_cast<const uint16_t*>(base) + i);
 }
 
+template <bool kWide>
 __device__ __forceinline__ void unpack8(const Raw8& r, int type, float (&x)[8]) {
-    if (type == GS_F32) {
-        x[0] = __uint_as_float(r.a.x);
-        x[1] = __uint_as_float(r.a.y);
-        x[2] = __uint_as_float(r.a.z);
-        x[3] = __uint_as_float(r.a.w);
-        x[4] = __uint_as_float(r.b.x);
-        x[5] = __uint_as_float(r.b.y);
-        x[6] = __uint_as_float(r.b.z);
-        x[7] = __uint_as_float(r.b.w);
-    } else {
-        const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    if (kWide) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(w[k]);
+    } else if (type == GS_BF16) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float2 f = unpack2(w[k], type);
+            x[2 * k] = __uint_as_float(w[k] << 16);
+            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
             x[2 * k] = f.x;
             x[2 * k + 1] = f.y;
         }
     }
+}
+
+__device__ __forceinline__ void unpack8(const Raw8& r, int type, float (&x)[8]) {
+    if (type == GS_F32)
+        unpack8<true>(r, type, x);
+    else
+        unpack8<false>(r, type, x);
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, int type) {
@@ -96,16 +110,36 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int type) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void store_vec8(void* base, int64_t i, int type, const float (&x)[8]) {
-    if (type == GS_F32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + i);
-        __stcs(p, make_float4(x[0], x[1], x[2], x[3]));
-        __stcs(p + 1, make_float4(x[4], x[5], x[6], x[7]));
+template <bool kStream>
+__device__ __forceinline__ void store16(void* p, uint4 x) {
+    if (kStream)
+        __stcs(static_cast<uint4*>(p), x);
+    else
+        *static_cast<uint4*>(p) = x;
+}
+
+template <bool kWide, bool kStream = false>
+__device__ __forceinline__ void store_vec8(void* p, int type, const float (&x)[8]) {
+    if (kWide) {
+#pragma unroll
+        for (int k = 0; k < 8; k += 4)
+            store16<kStream>(static_cast<float*>(p) + k,
+                             make_uint4(__float_as_uint(x[k]), __float_as_uint(x[k + 1]), __float_as_uint(x[k + 2]),
+                                        __float_as_uint(x[k + 3])));
+    } else if (type == GS_BF16) {
+        store16<kStream>(p, make_uint4(pack2(x[0], x[1], GS_BF16), pack2(x[2], x[3], GS_BF16),
+                                       pack2(x[4], x[5], GS_BF16), pack2(x[6], x[7], GS_BF16)));
     } else {
-        __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + i),
-               make_uint4(pack2(x[0], x[1], type), pack2(x[2], x[3], type), pack2(x[4], x[5], type),
-                          pack2(x[6], x[7], type)));
+        store16<kStream>(p, make_uint4(pack2(x[0], x[1], GS_F16), pack2(x[2], x[3], GS_F16),
+                                       pack2(x[4], x[5], GS_F16), pack2(x[6], x[7], GS_F16)));
     }
+}
+
+__device__ __forceinline__ void store_vec8(void* base, int64_t i, int type, const float (&x)[8]) {
+    if (type == GS_F32)
+        store_vec8<true>(static_cast<float*>(base) + i, type, x);
+    else
+        store_vec8<false>(static_cast<uint16_t*>(base) + i, type, x);
 }
 
 __device__ __forceinline__ float load_one(const void* base, int64_t off, int type) {
@@ -141,9 +175,14 @@ struct RowWalk {
     }
 };
 
-// Elements [i, i + 8) one by one: ragged ends, strided rows, odd alignment.
+// Elements [i, i + 8) where the end, rows or alignment of a tensor ask for single
+// accesses; ``vec``: 16-byte ones where all eight are inside.
 __device__ __forceinline__ void load_each8(const void* base, int64_t i, int64_t n, int64_t cols, int64_t stride,
-                                           int type, float (&x)[8]) {
+                                           int type, bool vec, float (&x)[8]) {
+    if (vec && i + kPerThread <= n) {
+        unpack8(load_raw8(base, i, type), type, x);
+        return;
+    }
     RowWalk w(i, cols, stride);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -153,7 +192,11 @@ __device__ __forceinline__ void load_each8(const void* base, int64_t i, int64_t 
 }
 
 __device__ __forceinline__ void store_each8(void* base, int64_t i, int64_t n, int64_t cols, int64_t stride, int type,
-                                            const float (&x)[8]) {
+                                            bool vec, const float (&x)[8]) {
+    if (vec && i + kPerThread <= n) {
+        store_vec8(base, i, type, x);
+        return;
+    }
     RowWalk w(i, cols, stride);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -162,26 +205,55 @@ __device__ __forceinline__ void store_each8(void* base, int64_t i, int64_t n, in
     }
 }
 
-// The tensor that chunk c belongs to.
+// A block's way through the chunks: it takes every gridDim-th group of successive
+// ones, in segments that lie in one tensor.  Neighbouring blocks work on
+// neighbouring memory, which DRAM prefers to as many distant streams as there are
+// blocks.
 template <int kCap>
-__device__ __forceinline__ int find_tensor(const TensorTable<kCap>& tab, int c) {
-    int lo = 0, hi = tab.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (tab.first[mid] <= c)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    return lo;
-}
+struct Segments {
+    const TensorTable<kCap>& tab;
+    int group, c, group_end, tensor;
 
-// This block's chunks [begin, end).
-template <int kCap>
-__device__ __forceinline__ void block_share(const TensorTable<kCap>& tab, int& begin, int& end) {
-    const int64_t total = tab.first[tab.count];
-    begin = (int)(total * blockIdx.x / gridDim.x);
-    end = (int)(total * (blockIdx.x + 1) / gridDim.x);
+    __device__ __forceinline__ explicit Segments(const TensorTable<kCap>& t) : tab(t) {
+        group = blockIdx.x;  // the grid has at most one block per group
+        enter();
+        int lo = 0, hi = tab.count - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (tab.first[mid] <= c)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        tensor = lo;
+    }
+    __device__ __forceinline__ void enter() {
+        c = group * tab.group;
+        group_end = min(c + tab.group, tab.first[tab.count]);
+    }
+    // Moves to the next segment: ``chunks`` of tensor ``tensor`` from its element ``from`` on.
+    __device__ __forceinline__ bool next(int& chunks, int64_t& from) {
+        if (c == group_end) {
+            group += gridDim.x;
+            if (group >= tab.groups) return false;
+            enter();
+        }
+        while (c >= tab.first[tensor + 1]) ++tensor;
+        chunks = min(group_end, tab.first[tensor + 1]) - c;
+        from = (int64_t)(c - tab.first[tensor]) * kChunk;
+        c += chunks;
+        return true;
+    }
+};
+
+// Of a segment's chunks, those in which this warp's 256 elements begin inside the
+// tensor (``mine``) and those in which they end inside it too (``whole``); i: the
+// thread's first element.
+__device__ __forceinline__ void warp_chunks(int64_t n, int64_t i, int chunks, int& mine, int& whole) {
+    constexpr int kWarp = 32 * kPerThread;
+    const int64_t left = n - (i - (threadIdx.x & 31) * kPerThread);
+    mine = left > 0 ? (int)min((int64_t)chunks, (left - 1) / kChunk + 1) : 0;
+    whole = left >= kWarp ? (int)min((int64_t)chunks, (left - kWarp) / kChunk + 1) : 0;
 }
 
 // Sum of ``n`` doubles by the whole block, the same in every thread and in every
@@ -208,7 +280,7 @@ __device__ __forceinline__ double sum_partials(const double* partials, int64_t n
 // ---------------------------------------------------------------- host side
 inline int type_bytes(int type) { return type == GS_F32 ? 4 : 2; }
 
-// Whether elements can be moved 16 bytes at a time from a multiple of 8 on.
+// Whether eight elements can be moved at a time from a multiple of 8 on.
 inline bool can_vector(const void* p, int64_t n, int64_t cols, int64_t stride) {
     return (cols >= n || stride == cols) && aligned16(p);
 }
@@ -254,7 +326,7 @@ inline int64_t fill_table(TensorTable<kCap>& tab, const gs_tensor* t, int64_t at
         const gs_tensor& s = t[at];
         if (s.n == 0) continue;
         const int64_t c = (s.n + kChunk - 1) / kChunk;
-        if (chunks + c > 0x7fffffff) break;
+        if (chunks + c > 0x7f000000) break;
         TensorEntry& e = tab.e[k];
         e.param = s.param;
         e.grad = const_cast<void*>(s.grad);
@@ -284,12 +356,17 @@ inline int64_t live_tensors(const gs_tensor* t, int64_t count) {
     return k;
 }
 
-// Blocks for a table: a wave of resident blocks, or fewer when there is less work.
+// Blocks for a table and the size of their groups: at most one wave of resident
+// blocks, and groups of at most ``most_group`` chunks, of the size that lets every
+// block take the same number of them.
 template <int kCap>
-inline int table_grid(const TensorTable<kCap>& tab, int blocks_per_sm) {
-    const int64_t most = (int64_t)sm_count() * blocks_per_sm;
+inline int table_grid(TensorTable<kCap>& tab, int blocks_per_sm, int most_group) {
     const int64_t chunks = tab.first[tab.count];
-    return (int)(chunks < most ? chunks : most);
+    const int64_t wave = (int64_t)sm_count() * blocks_per_sm;
+    const int64_t rounds = (chunks + wave * most_group - 1) / (wave * most_group);
+    tab.group = (int32_t)((chunks + wave * rounds - 1) / (wave * rounds));
+    tab.groups = (int32_t)((chunks + tab.group - 1) / tab.group);
+    return (int)(tab.groups < wave ? tab.groups : wave);
 }
 
 // Launch with programmatic stream serialisation (the kernel begins with
