@@ -141,6 +141,13 @@ class _on_device:
             torch.cuda.set_device(self.prev)
 
 
+def _dense(tensors: List) -> List:
+    """Dense tensors in the place of strided ones (anything else is left to the
+    checks)."""
+    return [t if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.is_contiguous() else t.contiguous()
+            for t in tensors]
+
+
 def _norm_partials(lib, entries: int, n: int, buffer: torch.Tensor, stream: int) -> int:
     count = ctypes.c_int64(0)
     _lib.check(lib.gs_grad_norm_partials(entries, n, buffer.data_ptr(), buffer.numel(), ctypes.byref(count), stream),
@@ -415,31 +422,24 @@ class FusedAdamW:
         their device, any of the three types; v must not be negative) and the
         step count.  With 8-bit moments values that the form holds are kept
         exactly and others are rounded with the step count's offsets."""
-        if set(m) != set(self.names) or set(v) != set(self.names):
+        if m.keys() != self.offsets.keys() or v.keys() != self.offsets.keys():
             raise ValueError("moments for exactly the optimizer's parameters are needed")
-        ml, vl = [m[k] for k in self.names], [v[k] for k in self.names]
-        for what, tensors in (("moment m", ml), ("moment v", vl)):
-            for name, x in zip(self.names, tensors):
-                _check_tensor(f"{what} of {name!r}", x)
-        if t is not None:
-            if t < 0:
-                raise ValueError(f"the step count must not be negative: {t}")
+        if t is not None and t < 0:
+            raise ValueError(f"the step count must not be negative: {t}")
+        ml, vl = list(map(m.__getitem__, self.names)), list(map(v.__getitem__, self.names))
         with _on_device(self.device):
-            entries = np.zeros(len(ml), _ENTRY)
-            entries["n"], entries["state"] = self._entries["n"], self._entries["state"]
+            entries = self._entries.copy()
             entries["cols"] = entries["param_stride"] = np.maximum(entries["n"], 1)
-            ml, vl = [x.contiguous() for x in ml], [x.contiguous() for x in vl]
-            self._with_grads(entries, self.names, self._shapes, ml, "moment m")
+            # a tensor's first place takes its m, the second its v
+            _, ml = self._with_grads(entries, self.names, self._shapes, _dense(ml), "moment m")
             entries["param"], entries["param_type"] = entries["grad"], entries["grad_type"]
-            self._with_grads(entries, self.names, self._shapes, vl, "moment v")
+            _, vl = self._with_grads(entries, self.names, self._shapes, _dense(vl), "moment v")
             if t is None:
                 t = self.t if self.state_bits == 8 else None
             else:
                 self._control[0].fill_(int(t))
             if self.state_bits == 32:
-                for slab, src in ((self.m, ml), (self.v, vl)):
-                    for dst, x in zip(self._views(slab).values(), src):
-                        dst.copy_(x)
+                torch._foreach_copy_(list(self._views(self.m).values()) + list(self._views(self.v).values()), ml + vl)
                 return
             lib = _lib.lib()
             _lib.check(lib.gs_moments8_quantize(entries.ctypes.data, len(entries), self.m.data_ptr(),
@@ -449,8 +449,7 @@ class FusedAdamW:
     def sync_master(self) -> None:
         """Takes the float32 master copies from the parameters again."""
         if self.master_slab is not None:
-            for dst, p in zip(self._views(self.master_slab).values(), self._params):
-                dst.copy_(p.detach())
+            torch._foreach_copy_(list(self._views(self.master_slab).values()), [p.detach() for p in self._params])
 
     def state_dict(self) -> Dict[str, object]:
         """A copy of the state: the moments in the form they are held in, the
@@ -550,40 +549,34 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
     return norm
 
 
-def _codes(tensors: List[torch.Tensor]):
-    """Type codes of the tensors: one number where they are all of one type."""
-    types = list(map(_dtype, tensors))
-    return TYPES[types[0]] if types.count(types[0]) == len(types) else np.array([TYPES[t] for t in types])
-
-
 def _clip_entries(gl: List[torch.Tensor], ol: List[torch.Tensor]) -> Optional[np.ndarray]:
     """The entries where every tensor is dense and none shares memory that
     another one writes; None where that takes a closer look."""
-    if not all(map(_is_contiguous, gl)):
-        return None
     n = len(gl)
-    words = np.zeros((n, _ENTRY.itemsize // 8), np.int64)  # the entries' fields, the two types sharing a word
-    size = words[:, 2]
-    size[:] = list(map(_numel, gl))
-    words[:, 4:7] = np.maximum(size, 1)[:, None]
-    g_type = o_type = _codes(gl)
-    g_ptr = words[:, 1]
-    g_ptr[:] = list(map(_data_ptr, gl))
-    o_ptr = words[:, 0]
-    if ol is gl:
-        o_ptr[:] = g_ptr
-    else:
-        if not (all(map(_is_contiguous, ol)) and all(map(_same_size, gl, ol))):
-            return None
-        o_type = _codes(ol)
-        o_ptr[:] = list(map(_data_ptr, ol))
-    words[:, 7] = o_type + g_type * (1 << 32)
-    o_end = o_ptr + size * (4 - 2 * (o_type != _lib.GS_F32))
-    order = o_ptr.argsort()
-    starts, ends = o_ptr[order], o_end[order]
-    if n > 1 and (ends[:-1] > starts[1:]).any():
+    apart = ol is not gl
+    every = gl + ol if apart else gl
+    if not all(map(_is_contiguous, every)) or (apart and not all(map(_same_size, gl, ol))):
         return None
-    if ol is not gl:
+    types = list(map(_dtype, every))
+    if types.count(types[0]) == len(types):
+        g_type = o_type = TYPES[types[0]]
+    else:
+        codes = np.array([TYPES[t] for t in types], np.int64)
+        g_type, o_type = codes[:n], codes[-n:]
+    ptr = np.array(list(map(_data_ptr, every)), np.int64)
+    g_ptr, o_ptr = ptr[:n], ptr[-n:]
+    size = np.array(list(map(_numel, gl)), np.int64)
+    words = np.zeros((n, _ENTRY.itemsize // 8), np.int64)  # the entries' fields, the two types sharing a word
+    words[:, 0], words[:, 1], words[:, 2] = o_ptr, g_ptr, size
+    words[:, 4:7] = np.maximum(size, 1)[:, None]
+    words[:, 7] = o_type + g_type * (1 << 32)
+    if n > 1 or apart:
+        o_end = o_ptr + size * (4 - 2 * (o_type != _lib.GS_F32))
+        order = o_ptr.argsort()
+        starts, ends = o_ptr[order], o_end[order]
+        if (ends[:-1] > starts[1:]).any():
+            return None
+    if apart:
         # a gradient may lie in its own output's memory, or in none: the last output that starts below its end
         g_end = g_ptr + size * (4 - 2 * (g_type != _lib.GS_F32))
         last = starts.searchsorted(g_end) - 1

@@ -88,12 +88,6 @@ __device__ __forceinline__ void adamw_prologue(const AdamWArgs& a, AdamWShared& 
     }
 }
 
-// The moments, every operation rounded by itself.
-__device__ __forceinline__ void moments_update(float g, float& m, float& v, const AdamWArgs& a) {
-    m = __fadd_rn(__fmul_rn(a.b1, m), __fmul_rn(a.omb1, g));
-    v = __fadd_rn(__fmul_rn(a.b2, v), __fmul_rn(a.omb2, __fmul_rn(g, g)));
-}
-
 // The parameter, with the hardware's approximate square root and reciprocal: 2
 // ulp each on the step, far below the rounding of the parameter it moves.  The
 // rounded forms take a slow path where m or v is a denormal, which is where the
@@ -116,10 +110,16 @@ struct AdamWTensor {
 
 __device__ __forceinline__ void update8(float (&p)[8], const float (&g)[8], float (&m)[8], float (&v)[8],
                                         const AdamWTensor& t, const AdamWArgs& a) {
+    const float_pair b1 = pair_of(a.b1, a.b1), omb1 = pair_of(a.omb1, a.omb1);
+    const float_pair b2 = pair_of(a.b2, a.b2), omb2 = pair_of(a.omb2, a.omb2), c = pair_of(t.gscale, t.gscale);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        moments_update(__fmul_rn(g[k], t.gscale), m[k], v[k], a);
+    for (int k = 0; k < 8; k += 2) {
+        // the moments, every operation rounded by itself
+        const float_pair gk = mul_pair(pair_of(g[k], g[k + 1]), c);
+        add_apart(mul_pair(b1, pair_of(m[k], m[k + 1])), mul_pair(omb1, gk), m[k], m[k + 1]);
+        add_apart(mul_pair(b2, pair_of(v[k], v[k + 1])), mul_pair(omb2, mul_pair(gk, gk)), v[k], v[k + 1]);
         p[k] = param_update(p[k], m[k], v[k], t.inv_sqrt_bc2, t.step, t.keep, a.eps);
+        p[k + 1] = param_update(p[k + 1], m[k + 1], v[k + 1], t.inv_sqrt_bc2, t.step, t.keep, a.eps);
     }
 }
 
@@ -161,8 +161,8 @@ __device__ __forceinline__ void adamw_chunks(const TensorEntry& e, const AdamWAr
         }
         unpack8<kWideP || kMaster>(rp, p_type, p);
         update8(p, g, m, v, t, a);
-        store_vec8<kWideP || kMaster>(p_at, p_type, p);
-        if (kMaster) store_vec8<false>(p16_at, p_type, p);
+        store_vec8<kWideP || kMaster, true>(p_at, p_type, p);
+        if (kMaster) store_vec8<false, true>(p16_at, p_type, p);
         if (kBits == 32) {
             store_vec8<true, true>(m_at, GS_F32, m);
             store_vec8<true, true>(v_at, GS_F32, v);

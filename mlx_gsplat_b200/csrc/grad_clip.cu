@@ -69,7 +69,8 @@ __global__ void __launch_bounds__(kMultiThreads) grad_norm_kernel(const __grid_c
             else
                 norm_chunks<false>(e, i, chunks, sum);
         }
-        for (; chunks > 0 && i < e.n; --chunks, i += kChunk) {
+        // a warp as one: its lanes may load for one another
+        for (; chunks > 0 && i - (threadIdx.x & 31) * kPerThread < e.n; --chunks, i += kChunk) {
             load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, e.grad_vec, g);
             sum += sum_squares8(g);
         }
@@ -133,7 +134,8 @@ __global__ void __launch_bounds__(kMultiThreads) grad_clip_kernel(const __grid_c
             else
                 clip_chunks<false>(e, f, i, chunks);
         }
-        for (; chunks > 0 && i < e.n; --chunks, i += kChunk) {
+        // a warp as one: its lanes may load for one another
+        for (; chunks > 0 && i - (threadIdx.x & 31) * kPerThread < e.n; --chunks, i += kChunk) {
             load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, e.grad_vec, g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) g[j] = __fmul_rn(g[j], f);

@@ -157,51 +157,108 @@ __device__ __forceinline__ void store_one(void* base, int64_t off, int type, flo
         static_cast<__half*>(base)[off] = __float2half_rn(x);
 }
 
-// Walks the storage offsets of consecutive elements of a tensor whose rows of
-// ``cols`` elements lie ``stride`` apart.
+// Storage offsets of every 32nd element of a tensor whose rows of ``cols`` elements
+// lie ``stride`` apart.
 struct RowWalk {
-    int64_t off, col, cols, skip;
+    int64_t off, col, cols, step, col_step, skip;
     __device__ __forceinline__ RowWalk(int64_t i, int64_t cols_, int64_t stride) : cols(cols_), skip(stride - cols_) {
         const int64_t row = (i | cols_) >> 32 ? i / cols_ : (int64_t)((uint32_t)i / (uint32_t)cols_);
         col = i - row * cols_;
         off = row * stride + col;
+        const int rows = cols_ < 32 ? 32 / (int)cols_ : 0;
+        col_step = 32 - rows * cols_;
+        step = rows * stride + col_step;
     }
     __device__ __forceinline__ void next() {
-        ++off;
-        if (++col == cols) {
-            col = 0;
+        off += step;
+        col += col_step;
+        if (col >= cols) {
+            col -= cols;
             off += skip;
         }
     }
 };
 
-// Elements [i, i + 8) where the end, rows or alignment of a tensor ask for single
-// accesses; ``vec``: 16-byte ones where all eight are inside.
-__device__ __forceinline__ void load_each8(const void* base, int64_t i, int64_t n, int64_t cols, int64_t stride,
-                                           int type, bool vec, float (&x)[8]) {
-    if (vec && i + kPerThread <= n) {
-        unpack8(load_raw8(base, i, type), type, x);
-        return;
-    }
-    RowWalk w(i, cols, stride);
+// Eight consecutive elements a lane of a warp's 256, where rows or alignment rule
+// wide accesses out: the warp loads and stores 32 neighbours at a time and turns
+// them round in shared memory.  Every lane takes part; ``i`` is the lane's first
+// element.  (Each lane by itself, eight accesses 32 bytes apart: a step over the
+// columns of a pool of 1M Gaussians takes 628 us instead of 560, with 8-bit moments
+// 513 instead of 431.)
+__device__ __forceinline__ float* warp_stage() {
+    __shared__ __align__(16) float stage[kMultiThreads / 32][32 * kPerThread];
+    return stage[threadIdx.x >> 5];
+}
+
+__device__ __forceinline__ void load_rows8(const void* base, int64_t i, int64_t n, int64_t cols, int64_t stride,
+                                           int type, float (&x)[8]) {
+    const int lane = threadIdx.x & 31;
+    const int64_t left = n - (i - lane * (kPerThread - 1));
+    RowWalk w(i - lane * (kPerThread - 1), cols, stride);
+    float y[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        x[k] = i + k < n ? load_one(base, w.off, type) : 0.0f;
+        y[k] = 32 * k < left ? load_one(base, w.off, type) : 0.0f;
         w.next();
+    }
+    float* s = warp_stage();
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[32 * k + lane] = y[k];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(s + kPerThread * lane + k);
+        x[k] = q.x;
+        x[k + 1] = q.y;
+        x[k + 2] = q.z;
+        x[k + 3] = q.w;
+    }
+}
+
+__device__ __forceinline__ void store_rows8(void* base, int64_t i, int64_t n, int64_t cols, int64_t stride, int type,
+                                            const float (&x)[8]) {
+    const int lane = threadIdx.x & 31;
+    float* s = warp_stage();
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 8; k += 4)
+        *reinterpret_cast<float4*>(s + kPerThread * lane + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+    __syncwarp();
+    const int64_t left = n - (i - lane * (kPerThread - 1));
+    RowWalk w(i - lane * (kPerThread - 1), cols, stride);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (32 * k < left) store_one(base, w.off, type, s[32 * k + lane]);
+        w.next();
+    }
+}
+
+// The same for any tensor: ``vec`` (of the whole tensor) for wide accesses, with
+// single ones at its end.
+__device__ __forceinline__ void load_each8(const void* base, int64_t i, int64_t n, int64_t cols, int64_t stride,
+                                           int type, bool vec, float (&x)[8]) {
+    if (!vec) {
+        load_rows8(base, i, n, cols, stride, type, x);
+    } else if (i + kPerThread <= n) {
+        unpack8(load_raw8(base, i, type), type, x);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = i + k < n ? load_one(base, i + k, type) : 0.0f;
     }
 }
 
 __device__ __forceinline__ void store_each8(void* base, int64_t i, int64_t n, int64_t cols, int64_t stride, int type,
                                             bool vec, const float (&x)[8]) {
-    if (vec && i + kPerThread <= n) {
+    if (!vec) {
+        store_rows8(base, i, n, cols, stride, type, x);
+    } else if (i + kPerThread <= n) {
         store_vec8(base, i, type, x);
-        return;
-    }
-    RowWalk w(i, cols, stride);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        if (i + k < n) store_one(base, w.off, type, x[k]);
-        w.next();
+        for (int k = 0; k < 8; ++k) {
+            if (i + k < n) store_one(base, i + k, type, x[k]);
+        }
     }
 }
 
