@@ -141,6 +141,14 @@ class _on_device:
             torch.cuda.set_device(self.prev)
 
 
+def _changed(tensors: List[torch.Tensor]) -> None:
+    """Tells autograd that the tensors were written."""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:  # inference tensors have no version
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def _dense(tensors: List) -> List:
     """Dense tensors in the place of strided ones (anything else is left to the
     checks)."""
@@ -169,7 +177,10 @@ class FusedAdamW:
     are when a gradient is not finite (a step with ``max_norm`` always does).
 
     Parameters may be strided rows (a pool's columns); they may not overlap.
-    The optimizer belongs to one stream at a time, as its parameters do."""
+    ``lr``, ``weight_decay``, ``beta1``, ``beta2``, ``eps``, ``max_norm`` and
+    ``skip_nonfinite`` may be changed between steps (a captured step keeps the
+    values it was captured with, but for a tensor ``lr``).  The optimizer
+    belongs to one stream at a time, as its parameters do."""
 
     def __init__(self, params: Dict[str, torch.Tensor], lr: Union[float, torch.Tensor] = 1e-3,
                  betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
@@ -208,7 +219,6 @@ class FusedAdamW:
         self.device = _check_cuda(self._params)
         self.beta1, self.beta2 = float(betas[0]), float(betas[1])
         self.eps = float(eps)
-        self.weight_decay = float(weight_decay)
         self.state_bits = state_bits
         self.skip_nonfinite = bool(skip_nonfinite)
         self.lr = lr
@@ -231,8 +241,9 @@ class FusedAdamW:
         e["param_stride"] = [s for _, s in self._rows]
         e["param_type"] = [TYPES[p.dtype] for p in self._params]
         e["lr_scale"] = [float((lr_scales or {}).get(k, 1.0)) for k in self.names]
-        e["decay"] = [self.weight_decay * float((decay_scales or {}).get(k, 1.0)) for k in self.names]
         self._entries, self._at = e, e.ctypes.data
+        self._decay_scales = np.array([float((decay_scales or {}).get(k, 1.0)) for k in self.names])
+        self.weight_decay = weight_decay
         dt = torch.float32 if state_bits == 32 else torch.uint8
         self.m = torch.zeros(self.slab_elements, dtype=dt, device=self.device)
         self.v = torch.zeros(self.slab_elements, dtype=dt, device=self.device)
@@ -250,6 +261,17 @@ class FusedAdamW:
         self._partials: Optional[torch.Tensor] = None
         if max_norm is not None or skip_nonfinite:
             self._partials_buffer(_lib.lib())
+
+    @property
+    def weight_decay(self) -> float:
+        return self._weight_decay
+
+    @weight_decay.setter
+    def weight_decay(self, value: float) -> None:
+        if not (math.isfinite(value) and value >= 0.0):
+            raise ValueError(f"weight_decay must not be negative: {value}")
+        self._weight_decay = float(value)
+        self._entries["decay"] = self._weight_decay * self._decay_scales
 
     # ------------------------------------------------------------------ checks
     def _lr_value(self) -> Tuple[float, Optional[int]]:
@@ -304,7 +326,8 @@ class FusedAdamW:
         ``shapes``); returns the entries (a copy where their rows had to change)
         and the tensors that must outlive the launch."""
         try:
-            types = list(map(TYPES.__getitem__, map(_dtype, grads)))
+            types = list(map(_dtype, grads))
+            codes = list(map(TYPES.__getitem__, types)) if types.count(types[0]) != len(types) else TYPES[types[0]]
             same = list(map(_shape, grads)) == shapes
             here = set(map(_device_index, grads)) == {self.device.index}
             dense = all(map(_is_contiguous, grads))
@@ -319,7 +342,7 @@ class FusedAdamW:
                     raise ValueError(f"{what} of {name!r} has shape {tuple(g.shape)}, not {tuple(s)}")
         if not here:
             raise ValueError(f"every {what} must be on {self.device}")
-        entries["grad_type"] = types
+        entries["grad_type"] = codes
         entries["grad_stride"] = entries["cols"]
         if not dense:
             entries, grads = entries.copy(), list(grads)
@@ -384,7 +407,7 @@ class FusedAdamW:
                 s.norm_out = norm.data_ptr()
             _lib.check(lib.gs_adamw_step(at, len(entries), self._state, s, stream), "adamw step")
             del keep
-        torch.autograd.graph.increment_version(params)
+        _changed(params)
         return norm
 
     # ------------------------------------------------------------------ state
@@ -545,7 +568,7 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
         count = _norm_partials(lib, at, n, partials, stream)
         _lib.check(lib.gs_clip_gradients(at, n, partials.data_ptr(), count, max_norm, norm.data_ptr(), stream),
                    "clip gradients")
-    torch.autograd.graph.increment_version(ol)
+    _changed(ol)
     return norm
 
 

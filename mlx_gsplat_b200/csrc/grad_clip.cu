@@ -9,7 +9,9 @@
 // partial sum, every consumer adds them in index order), so a run repeats bit for
 // bit.  Finding the norm has to read every gradient before the first may be
 // scaled; only gradients that still lie in the 126 MB L2 are not read from
-// memory twice.
+// memory twice.  59M float32: norm 36 us (of measured copy rate: 100 %), norm and
+// clipping into other tensors 119 us (three passes: 91 %); bfloat16 is held up by
+// the conversions to 64 bits (norm 22 us, 81 %).
 #include <math.h>
 
 #include "multi_tensor.cuh"

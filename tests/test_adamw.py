@@ -118,6 +118,23 @@ def test_bad_clipping():
         clip_gradients([big[:8]], 1.0, out=[big[:8]])
 
 
+def test_calls_are_made_on_the_tensors_device(monkeypatch):
+    """Launches go to the device that is current: it is switched for a call on
+    another one's tensors, and switched back, also after an error."""
+    from mlx_gsplat_b200.adamw import _on_device
+    now = [0]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "set_device", lambda i: now.__setitem__(0, i))
+    for index in (0, 3):
+        with _on_device(torch.device("cuda", index)):
+            assert now == [index]
+        assert now == [0]
+        with pytest.raises(KeyError):
+            with _on_device(torch.device("cuda", index)):
+                raise KeyError
+        assert now == [0]
+
+
 # ---------------------------------------------------------------- C ABI checks (no CUDA call is reached)
 def _entry(**kw):
     e = np.zeros(1, _ENTRY)

@@ -422,6 +422,61 @@ def test_two_captured_clips_do_not_share_workspace():
         assert abs(float(o.double().norm()) - 1.0) < 1e-6
 
 
+def test_two_optimizers_on_two_streams():
+    shapes = {"a": (70_001,), "b": (333, 3)}
+    results = []
+    for apart in (False, True):
+        params = [tensors(1 + k, shapes, F32) for k in range(2)]
+        opts = [FusedAdamW(p, state_bits=8, max_norm=0.1) for p in params]
+        grads = [tensors(7 + k, shapes, BF16) for k in range(2)]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()] if apart else [torch.cuda.current_stream()] * 2
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s, o, g in zip(streams, opts, grads):
+                with torch.cuda.stream(s):
+                    o.step(g)
+        torch.cuda.synchronize()
+        results.append([x for p, o in zip(params, opts) for x in (*p.values(), o.m, o.v, o.m_exp, o.v_exp)])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+def test_one_gradient_for_two_parameters_and_changed_settings():
+    shapes = {"a": (300,), "b": (300,)}
+    params = tensors(1, shapes, F32)
+    opt = FusedAdamW(params, weight_decay=0.0)
+    ref = Reference(opt, params)
+    g = torch.randn(300, device=DEV)
+    opt.step({"a": g, "b": g})
+    ref.check({"a": g, "b": g})
+    opt.lr, opt.weight_decay, opt.eps, opt.beta1 = 0.03, 0.5, 1e-4, 0.5
+    opt.step({"a": g, "b": g})
+    # the oracle's correction uses the betas of the step, as the kernel's does
+    ref.check({"a": g, "b": g}, lr=0.03)
+    with pytest.raises(ValueError):
+        opt.weight_decay = -1.0
+    opt.beta2 = 1.0
+    with pytest.raises(RuntimeError, match="betas"):
+        opt.step({"a": g, "b": g})
+
+
+def test_masters_follow_parameters_when_asked():
+    params = tensors(1, {"a": (300,)}, BF16)
+    opt = FusedAdamW(params, master_weights=True)
+    params["a"].mul_(3.0)
+    opt.sync_master()
+    assert torch.equal(opt._views(opt.master_slab)["a"], params["a"].float())
+
+
+def test_inference_tensors():
+    with torch.inference_mode():
+        g, p = torch.ones(100, device=DEV), torch.zeros(100, device=DEV)
+        clip_gradients([g], 1.0)
+        FusedAdamW({"a": p}, lr=1.0, weight_decay=0.0).step({"a": g})
+    # each gradient is 0.1 up to two roundings, and the first step moves by lr (up to 16 roundings and eps)
+    assert ((g - 0.1).abs() <= 0.1 * 3 * 2.0 ** -24).all()
+    assert ((p + 1.0).abs() <= 20 * 2.0 ** -24 + 1e-7).all()
+
+
 def test_replaced_parameter_memory():
     params = {"a": torch.randn(100, device=DEV), "b": torch.randn(30, device=DEV)}
     opt = FusedAdamW(params)
