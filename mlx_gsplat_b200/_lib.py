@@ -192,8 +192,16 @@ def check(status: int, what: str = "") -> None:
     raise GsplatError(f"{what} failed ({status}): {msg}")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: Optional[torch.device] = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The device's current stream (without building a Stream object where
+    torch offers its address, which is most of a small call's host time)."""
+    if _raw_stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    index = None if device is None else device.index
+    return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

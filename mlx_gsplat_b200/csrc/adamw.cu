@@ -117,14 +117,21 @@ struct AdamWTensor {
 
 __device__ __forceinline__ void update8(float (&p)[8], const float (&g)[8], float (&m)[8], float (&v)[8],
                                         const AdamWTensor& t, const AdamWArgs& a) {
-    const float_pair b1 = pair_of(a.b1, a.b1), omb1 = pair_of(a.omb1, a.omb1);
-    const float_pair b2 = pair_of(a.b2, a.b2), omb2 = pair_of(a.omb2, a.omb2), c = pair_of(t.gscale, t.gscale);
+    const float2 b1 = make_float2(a.b1, a.b1), omb1 = make_float2(a.omb1, a.omb1);
+    const float2 b2 = make_float2(a.b2, a.b2), omb2 = make_float2(a.omb2, a.omb2);
+    const float2 c = make_float2(t.gscale, t.gscale);
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
-        // the moments, every operation rounded by itself
-        const float_pair gk = mul_pair(pair_of(g[k], g[k + 1]), c);
-        add_apart(mul_pair(b1, pair_of(m[k], m[k + 1])), mul_pair(omb1, gk), m[k], m[k + 1]);
-        add_apart(mul_pair(b2, pair_of(v[k], v[k + 1])), mul_pair(omb2, mul_pair(gk, gk)), v[k], v[k + 1]);
+        // The moments, every operation rounded by itself: the products of two elements in one instruction, the sums
+        // in single ones, because packed products and sums are joined into fused ones even where both name their
+        // rounding.
+        const float2 gk = __fmul2_rn(make_float2(g[k], g[k + 1]), c);
+        const float2 ma = __fmul2_rn(b1, make_float2(m[k], m[k + 1])), mb = __fmul2_rn(omb1, gk);
+        const float2 va = __fmul2_rn(b2, make_float2(v[k], v[k + 1])), vb = __fmul2_rn(omb2, __fmul2_rn(gk, gk));
+        m[k] = __fadd_rn(ma.x, mb.x);
+        m[k + 1] = __fadd_rn(ma.y, mb.y);
+        v[k] = __fadd_rn(va.x, vb.x);
+        v[k + 1] = __fadd_rn(va.y, vb.y);
         p[k] = param_update(p[k], m[k], v[k], t.inv_sqrt_bc2, t.step, t.keep, a.eps);
         p[k + 1] = param_update(p[k + 1], m[k + 1], v[k + 1], t.inv_sqrt_bc2, t.step, t.keep, a.eps);
     }

@@ -31,42 +31,6 @@
 
 namespace gs {
 
-// Two float32 operations in one instruction, each rounded by itself.
-typedef unsigned long long float_pair;
-
-__device__ __forceinline__ float_pair pair_of(float a, float b) {
-    float_pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-
-__device__ __forceinline__ void split_pair(float_pair r, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-
-__device__ __forceinline__ float_pair mul_pair(float_pair a, float_pair b) {
-    float_pair r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
-// a + b, where a or b is a product that keeps its own rounding: in single
-// instructions, because the assembler joins packed products and sums into fused
-// ones even when both name their rounding.
-__device__ __forceinline__ void add_apart(float_pair a, float_pair b, float& x, float& y) {
-    float a0, a1, b0, b1;
-    split_pair(a, a0, a1);
-    split_pair(b, b0, b1);
-    x = __fadd_rn(a0, b0);
-    y = __fadd_rn(a1, b1);
-}
-
-__device__ __forceinline__ float_pair add_pair_rz(float_pair a, float_pair b) {
-    float_pair r;
-    asm("add.rz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 constexpr uint32_t kDitherElement = 0x9E3779B1u;  // odd, close to 2^32 / golden ratio
 constexpr uint32_t kDitherStep = 0x6A09E667u;     // fractional bits of sqrt(2)
 constexpr int kMomentTopM = 15, kMomentTopV = 31;
@@ -89,9 +53,13 @@ struct MomentScale {
 };
 
 __device__ __forceinline__ void scale8(float (&x)[8], float f) {
-    const float_pair ff = pair_of(f, f);
+    const float2 ff = make_float2(f, f);
 #pragma unroll
-    for (int k = 0; k < 8; k += 2) split_pair(mul_pair(pair_of(x[k], x[k + 1]), ff), x[k], x[k + 1]);
+    for (int k = 0; k < 8; k += 2) {
+        const float2 y = __fmul2_rn(make_float2(x[k], x[k + 1]), ff);
+        x[k] = y.x;
+        x[k + 1] = y.y;
+    }
 }
 
 // Eight codes (two words) to values; ``e`` the block's exponent byte (255: no
@@ -148,11 +116,11 @@ __device__ __forceinline__ void encode8(const uint32_t (&a)[8], uint32_t w, uint
     e = min(max(most >> 23, kMomentMinExp), 255u);
     const uint32_t low = (e - (kTop - 1)) << 23;  // L, the smallest magnitude with exponent field 1
     const int base = (int)(e - kTop) << 3;
-    const float_pair low2 = pair_of(__uint_as_float(low), __uint_as_float(low));
+    const float2 low2 = make_float2(__uint_as_float(low), __uint_as_float(low));
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
-        float fixed[2];
-        split_pair(add_pair_rz(pair_of(__uint_as_float(a[k]), __uint_as_float(a[k + 1])), low2), fixed[0], fixed[1]);
+        const float2 fixed2 = __fadd2_rz(make_float2(__uint_as_float(a[k]), __uint_as_float(a[k + 1])), low2);
+        const float fixed[2] = {fixed2.x, fixed2.y};
 #pragma unroll
         for (int j = k; j < k + 2; ++j) {
             const uint32_t z = (uint32_t)max((int)a[j], (int)(__float_as_uint(fixed[j - k]) - (1u << 23)));

@@ -118,6 +118,35 @@ def test_bad_clipping():
         clip_gradients([big[:8]], 1.0, out=[big[:8]])
 
 
+@pytest.mark.parametrize("count", [3, 16, 17, 40])  # plain loops, array operations
+def test_entries_of_dense_tensors(count):
+    """The dense tensors' entries, and the cases that take a closer look."""
+    from mlx_gsplat_b200.adamw import _clip_entries
+    back = torch.zeros(100 * count)
+    gl = [back[100 * k:100 * k + 90 + k % 3] for k in range(count)]
+    ol = [torch.zeros(g.shape, dtype=torch.bfloat16 if k % 2 else torch.float32) for k, g in enumerate(gl)]
+    for out in (gl, ol):
+        e = _clip_entries(gl, out)
+        assert e["grad"].tolist() == [g.data_ptr() for g in gl] and e["param"].tolist() == [o.data_ptr() for o in out]
+        for name in ("n", "cols", "param_stride", "grad_stride"):
+            assert e[name].tolist() == [g.numel() for g in gl]
+        assert e["grad_type"].tolist() == [0] * count
+        assert e["param_type"].tolist() == [int(o.dtype == torch.bfloat16) for o in out]
+    same = list(gl)
+    assert _clip_entries(gl, same) is not None  # each in its own memory
+    assert _clip_entries(gl, same[1:] + same[:1]) is None  # in others'
+    assert _clip_entries(gl, ol[:-1] + [ol[0].view(-1)]) is None  # written twice
+    assert _clip_entries(gl[:-1] + [gl[0]], gl[:-1] + [gl[0]]) is None
+    assert _clip_entries(gl, ol[:-1] + [back[100 * count - 50:].new_zeros(gl[-1].shape)]) is not None
+    assert _clip_entries(gl, ol[:-1] + [back[50:50 + gl[-1].numel()]]) is None  # part of another gradient
+    assert _clip_entries(gl, ol[:-1] + [torch.zeros(2 * gl[-1].numel())[::2]]) is None  # strided
+    assert _clip_entries(gl, ol[:-1] + [torch.zeros(gl[-1].numel(), 1)]) is None  # another shape
+    assert _clip_entries(gl[:-1] + [gl[-1].view(torch.bfloat16)[:9]], gl[:-1] + [gl[-1][:9]]) is None  # another type
+    zero = [torch.zeros(0)] * count
+    e = _clip_entries(zero, zero)
+    assert e is None or not e["n"].any()
+
+
 def test_calls_are_made_on_the_tensors_device(monkeypatch):
     """Launches go to the device that is current: it is switched for a call on
     another one's tensors, and switched back, also after an error."""

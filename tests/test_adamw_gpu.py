@@ -228,6 +228,19 @@ def test_clip_strided_and_repeated_gradients():
     assert torch.equal(slab[:, 6:], before[:, 6:]) and not torch.equal(slab[:, 1:4], before[:, 1:4])
 
 
+@pytest.mark.parametrize("count", [24, 25, 500])
+def test_clip_more_tensors_than_a_table(count):
+    rng = np.random.default_rng(count)
+    shapes = {f"x{i}": (int(n),) for i, n in enumerate(rng.integers(0, 5000, count))}
+    grads = tensors(3, shapes, F32)
+    before = {k: g.clone() for k, g in grads.items()}
+    exact = math.sqrt(sum(float(g.double().square().sum()) for g in grads.values()))
+    assert abs(float(clip_gradients(grads, 0.1 * exact)) - exact) <= 2.0 ** -24 * 1.01 * exact
+    for k, g in grads.items():
+        want = before[k].double() * 0.1
+        assert ((g.double() - want).abs() <= 2.0 ** -23 * 1.01 * want.abs()).all(), k
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_not_finite_gradients_are_left(bad):
     g = {"a": torch.randn(5000, device=DEV), "b": torch.zeros(0, device=DEV), "c": torch.randn(3, device=DEV)}
