@@ -13,6 +13,7 @@ import torch
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libgsplat_b200.so")
+TENSORS_PATH = os.path.join(PKG, "libgsplat_tensors.so")
 
 GS_OK, GS_ERR_INVALID, GS_ERR_CUDA, GS_ERR_CAPACITY = 0, 1, 2, 3
 GS_ADAM_FUSED, GS_ADAM_PURE, GS_ADAM_EXACT = 0, 1, 0x100
@@ -170,6 +171,24 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         f.argtypes = args
     _LIB = lib
     return lib
+
+
+_TENSORS: Optional[ctypes.PyDLL] = None
+
+
+def tensors() -> Optional[ctypes.PyDLL]:
+    """The helper that reads tensors' metadata natively (``csrc/tensors.cpp``;
+    called with the GIL held), or None where it was not built: the callers' own
+    checks in Python then do the same."""
+    global _TENSORS
+    if _TENSORS is None and os.path.exists(TENSORS_PATH):
+        dll = ctypes.PyDLL(TENSORS_PATH)
+        obj, size = ctypes.py_object, ctypes.c_ssize_t
+        dll.gst_fill.argtypes = [obj, obj, obj, obj, c_vp, size, ctypes.c_int]
+        dll.gst_params_unmoved.argtypes = [obj, c_vp, size]
+        dll.gst_clip.argtypes = [obj, obj, c_vp, size, ctypes.POINTER(ctypes.c_int)]
+        _TENSORS = dll
+    return _TENSORS
 
 
 def exported_names():

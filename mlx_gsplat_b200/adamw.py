@@ -370,25 +370,31 @@ class FusedAdamW:
         norm of the scaled gradients before clipping as a device scalar when
         ``max_norm`` or ``skip_nonfinite`` asks for it, else None."""
         lib = _lib.lib()
-        if grads is None:
-            found = [p.grad for p in self._params]
-        else:
-            found = list(map(grads.get, self.names))
-            if len(grads) != len(found) and not grads.keys() <= self.offsets.keys():
-                raise ValueError(f"no parameter named {sorted(set(grads) - set(self.names))}")
         if not math.isfinite(grad_scale):
             raise ValueError(f"grad_scale must be finite: {grad_scale}")
         lr, lr_device = self._lr_value()
         limit = self._norm_limit()
-        if list(map(_data_ptr, self._params)) != self._ptrs:
-            self._refresh()
         names, shapes, params, entries = self.names, self._shapes, self._params, self._entries
-        if any(map(_is_none, found)):
-            if grads is not None and not grads.keys() <= self.offsets.keys():
-                raise ValueError(f"no parameter named {sorted(set(grads) - set(self.names))}")
-            on = [k for k, g in enumerate(found) if g is not None]
-            entries = entries[on]
-            names, shapes, params, found = ([x[k] for k in on] for x in (names, shapes, params, found))
+        native = _lib.tensors()
+        # every gradient there, dense and as expected: the table is filled natively
+        filled = native is not None and \
+            not native.gst_fill(grads, names, params, self._aliases, self._at, len(params), self.device.index) and \
+            not native.gst_params_unmoved(params, self._at, len(params))
+        if not filled:
+            if grads is None:
+                found = [p.grad for p in params]
+            else:
+                found = list(map(grads.get, names))
+            if list(map(_data_ptr, params)) != self._ptrs:
+                self._refresh()
+            none = any(map(_is_none, found))
+            if (none or (grads is not None and len(grads) != len(found))) and grads is not None and \
+                    not grads.keys() <= self.offsets.keys():
+                raise ValueError(f"no parameter named {sorted(set(grads) - set(names))}")
+            if none:
+                on = [k for k, g in enumerate(found) if g is not None]
+                entries = entries[on]
+                names, shapes, params, found = ([x[k] for k in on] for x in (names, shapes, params, found))
         with_norm = self.max_norm is not None or self.skip_nonfinite
         norm = None
         with _on_device(self.device):
@@ -396,7 +402,8 @@ class FusedAdamW:
                 norm = torch.empty((), dtype=torch.float32, device=self.device)
             if not self._elements_in(entries):
                 return norm.zero_() if with_norm else None
-            entries, keep = self._with_grads(entries, names, shapes, found)
+            if not filled:
+                entries, keep = self._with_grads(entries, names, shapes, found)
             at = self._at if entries is self._entries else entries.ctypes.data
             stream = _lib.stream_ptr(self.device)
             s = _lib.GsAdamWSettings(lr, self.beta1, self.beta2, self.eps, grad_scale, lr_device, None, 0, limit, None)
@@ -406,8 +413,9 @@ class FusedAdamW:
                 s.norm_partials = buffer.data_ptr()
                 s.norm_out = norm.data_ptr()
             _lib.check(lib.gs_adamw_step(at, len(entries), self._state, s, stream), "adamw step")
+        if not filled:
             del keep
-        _changed(params)
+            _changed(params)
         return norm
 
     # ------------------------------------------------------------------ state
@@ -454,9 +462,9 @@ class FusedAdamW:
             entries = self._entries.copy()
             entries["cols"] = entries["param_stride"] = np.maximum(entries["n"], 1)
             # a tensor's first place takes its m, the second its v
-            _, ml = self._with_grads(entries, self.names, self._shapes, _dense(ml), "moment m")
+            ml = self._fill_dense(entries, ml, "moment m")
             entries["param"], entries["param_type"] = entries["grad"], entries["grad_type"]
-            _, vl = self._with_grads(entries, self.names, self._shapes, _dense(vl), "moment v")
+            vl = self._fill_dense(entries, vl, "moment v")
             if t is None:
                 t = self.t if self.state_bits == 8 else None
             else:
@@ -468,6 +476,13 @@ class FusedAdamW:
             _lib.check(lib.gs_moments8_quantize(entries.ctypes.data, len(entries), self.m.data_ptr(),
                                                 self.v.data_ptr(), self.m_exp.data_ptr(), self.v_exp.data_ptr(),
                                                 int(t), _lib.stream_ptr(self.device)), "8-bit moments")
+
+    def _fill_dense(self, entries: np.ndarray, tensors: List[torch.Tensor], what: str) -> List[torch.Tensor]:
+        native = _lib.tensors()
+        if native is None or native.gst_fill(tensors, None, None, self._aliases, entries.ctypes.data, len(tensors),
+                                             self.device.index):
+            _, tensors = self._with_grads(entries, self.names, self._shapes, _dense(tensors), what)
+        return tensors
 
     def sync_master(self) -> None:
         """Takes the float32 master copies from the parameters again."""
@@ -548,8 +563,11 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
         raise ValueError("no gradients")
     if out is None:
         ol = gl
+    entries, index = np.zeros(len(gl), _ENTRY), ctypes.c_int(-1)
+    native = _lib.tensors()
+    filled = native is not None and not native.gst_clip(gl, ol, entries.ctypes.data, len(gl), ctypes.byref(index))
     try:
-        entries = _clip_entries(gl, ol)
+        entries = entries if filled else _clip_entries(gl, ol)
     except (KeyError, AttributeError, TypeError, RuntimeError):
         for name, g, o in zip(names, gl, ol):
             _check_tensor(f"gradient {name!r}", g)
@@ -557,7 +575,7 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
         raise
     if entries is None:
         entries, gl = _clip_entries_strided(names, gl, ol)
-    device = _check_cuda(gl + ol)
+    device = torch.device("cuda", index.value) if filled else _check_cuda(gl + ol)
     lib = _lib.lib()
     with _on_device(device):
         norm = torch.empty((), dtype=torch.float32, device=device)
@@ -568,7 +586,8 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
         count = _norm_partials(lib, at, n, partials, stream)
         _lib.check(lib.gs_clip_gradients(at, n, partials.data_ptr(), count, max_norm, norm.data_ptr(), stream),
                    "clip gradients")
-    _changed(ol)
+    if not filled:
+        _changed(ol)
     return norm
 
 

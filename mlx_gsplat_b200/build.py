@@ -2,7 +2,9 @@
 
 Usage: ``python -m mlx_gsplat_b200.build`` (or ``build()`` from Python).
 The library is a plain C ABI (``include/gsplat_b200.h``) loaded with ctypes;
-no PyTorch headers are involved.
+no PyTorch headers are involved.  Beside it ``libgsplat_tensors.so``
+(``csrc/tensors.cpp``, g++ with torch's headers) reads torch tensors' metadata
+for the many-tensor calls; it holds no kernels.
 """
 from __future__ import annotations
 
@@ -18,6 +20,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libgsplat_b200.so")
+TENSORS_SRC = os.path.join(CSRC, "tensors.cpp")
+TENSORS_LIB = os.path.join(PKG, "libgsplat_tensors.so")
 BUILD_DIR = os.path.join(PKG, "_build")
 
 NVCC_FLAGS = [
@@ -38,11 +42,31 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
 
 
+def build_tensors() -> str:
+    """Compile the tensor helper against the installed torch."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_paths()["include"]]
+    tmp = TENSORS_LIB + ".tmp"
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in includes),
+           "-I", INCLUDE, TENSORS_SRC, "-o", tmp, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
+           "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for tensors.cpp:\n" + r.stderr)
+    os.replace(tmp, TENSORS_LIB)
+    return TENSORS_LIB
+
+
 def _stale(objs, srcs) -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(TENSORS_LIB):
         return True
-    t = os.path.getmtime(LIB)
-    deps = srcs + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TENSORS_LIB))
+    deps = srcs + [TENSORS_SRC] + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
     return any(os.path.getmtime(d) > t for d in deps)
 
 
@@ -64,7 +88,9 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
         return r.stderr
 
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+        tensors = ex.submit(build_tensors)
         logs = list(ex.map(compile_one, zip(srcs, objs)))
+        tensors.result()
     if verbose:
         for s, log in zip(srcs, logs):
             if log.strip():

@@ -227,6 +227,20 @@ def test_other_entries_refuse_and_skip_nothing_to_do():
     assert lib.gs_moments8_dequantize(None, None, None, None, 0, 0, None, None, None) == 0
 
 
+def test_native_reader_leaves_host_tensors_alone():
+    native = _lib.tensors()
+    if native is None:
+        pytest.skip("helper not built")
+    e, device, t = np.zeros(1, _ENTRY), ctypes.c_int(-1), torch.zeros(3)
+    for items in ([t], {"a": t}, None, (t,), [t, t], 3):
+        assert native.gst_fill(items, ["a"], [t], [t], e.ctypes.data, 1, 0) == 1
+    assert native.gst_clip([t], [t], e.ctypes.data, 1, ctypes.byref(device)) == 1
+    assert native.gst_clip([], [], e.ctypes.data, 0, ctypes.byref(device)) == 1
+    assert native.gst_params_unmoved([t], e.ctypes.data, 1) == 1 and t._version == 0
+    e["param"] = t.data_ptr()
+    assert native.gst_params_unmoved([t], e.ctypes.data, 1) == 0 and t._version == 1
+
+
 # ---------------------------------------------------------------- the 8-bit form
 def test_every_code_is_kept():
     """A block of values on the grid is coded back to itself at any step."""

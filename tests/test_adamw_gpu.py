@@ -7,9 +7,9 @@ import numpy as np
 import pytest
 import torch
 
-from mlx_gsplat_b200 import (FusedAdamW, FusedMLXAdam, PointerStableChunkedAllocator, clip_gradients,
+from mlx_gsplat_b200 import (_lib, FusedAdamW, FusedMLXAdam, PointerStableChunkedAllocator, clip_gradients,
                              frustum_culling_mlx, rasterize_gaussians_mlx, synthetic)
-from mlx_gsplat_b200.adamw import BLOCK
+from mlx_gsplat_b200.adamw import _ENTRY, BLOCK, _clip_entries
 from oracle import adamw as oadamw
 
 pytestmark = pytest.mark.gpu
@@ -18,6 +18,16 @@ F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 HALF_STEP = {F32: 0.0, BF16: 2.0 ** -8, F16: 2.0 ** -11}  # a rounding to nearest, relative
 TINY = {F32: 0.0, BF16: 2.0 ** -134, F16: 2.0 ** -25}     # and below the normal range
 SIZES = [1, 7, 8, 9, 255, 256, 257, 0, 2047, 2048, 2049, 5003]
+
+
+@pytest.fixture(params=[True, False], ids=["native", "python"])
+def reader(request, monkeypatch):
+    """The tensors' metadata read natively, or by the checks in Python."""
+    if not request.param:
+        monkeypatch.setattr(_lib, "tensors", lambda: None)
+    else:
+        assert _lib.tensors() is not None
+    return request.param
 
 
 def tensors(seed, shapes, dtype, scale=1.0, sparse=0.0):
@@ -98,7 +108,7 @@ def test_step_matches_oracle(bits, ptype, gtype, master):
                   master=master)
 
 
-def test_mixed_types_in_one_step_and_grad_scale():
+def test_mixed_types_in_one_step_and_grad_scale(reader):
     shapes = {"a": (33, 5), "b": (2050,), "c": (7, 11, 13), "d": ()}
     params = {**tensors(1, {"a": shapes["a"], "d": ()}, F32), **tensors(2, {"b": shapes["b"]}, BF16),
               **tensors(3, {"c": shapes["c"]}, F16)}
@@ -113,7 +123,7 @@ def test_mixed_types_in_one_step_and_grad_scale():
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-def test_strided_rows_leave_their_surroundings(bits):
+def test_strided_rows_leave_their_surroundings(bits, reader):
     """Columns of one slab (a pool's views), an offset view and strided gradients."""
     slab = torch.randn(301, 20, device=DEV)
     back = torch.randn(4000, device=DEV)
@@ -138,7 +148,7 @@ def test_strided_rows_leave_their_surroundings(bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-def test_broadcast_gradients_and_missing_ones(bits):
+def test_broadcast_gradients_and_missing_ones(bits, reader):
     shapes = {"a": (300,), "b": (40, 9), "c": (3,)}
     params = {k: p.requires_grad_(True) for k, p in tensors(1, shapes, F32).items()}
     opt = FusedAdamW(params, state_bits=bits)
@@ -157,7 +167,7 @@ def test_broadcast_gradients_and_missing_ones(bits):
 
 
 @pytest.mark.parametrize("count", [25, 368, 369, 900])
-def test_more_tensors_than_a_table(count):
+def test_more_tensors_than_a_table(count, reader):
     rng = np.random.default_rng(count)
     shapes = {f"x{i}": (int(n),) for i, n in enumerate(rng.integers(0, 700, count))}
     params = tensors(1, shapes, F32)
@@ -174,7 +184,7 @@ def test_more_tensors_than_a_table(count):
 # ---------------------------------------------------------------- norm and clipping
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("scale", [1e-12, 1.0, 0.25, 1e12])
-def test_clip_gradients(dtype, scale):
+def test_clip_gradients(dtype, scale, reader):
     if dtype == F16 and scale != 1.0:
         scale = {1e-12: 1e-3, 0.25: 0.25, 1e12: 30.0}[scale]
     shapes = {f"x{i}": (n,) for i, n in enumerate(SIZES + [100_001])}
@@ -208,7 +218,7 @@ def test_clip_gradients(dtype, scale):
     assert all(torch.equal(grads[k], out[k]) for k in shapes)
 
 
-def test_clip_strided_and_repeated_gradients():
+def test_clip_strided_and_repeated_gradients(reader):
     slab = torch.randn(50, 12, device=DEV)
     same = torch.randn(77, device=DEV)
     grads = [slab[:, 1:4], slab[:, 5:6], same, same, torch.randn(6, 50, device=DEV).t()]
@@ -229,7 +239,7 @@ def test_clip_strided_and_repeated_gradients():
 
 
 @pytest.mark.parametrize("count", [24, 25, 500])
-def test_clip_more_tensors_than_a_table(count):
+def test_clip_more_tensors_than_a_table(count, reader):
     rng = np.random.default_rng(count)
     shapes = {f"x{i}": (int(n),) for i, n in enumerate(rng.integers(0, 5000, count))}
     grads = tensors(3, shapes, F32)
@@ -314,7 +324,7 @@ def test_not_finite_values_stay_in_their_elements():
 
 # ---------------------------------------------------------------- the 8-bit form
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-def test_load_moments_matches_oracle(dtype):
+def test_load_moments_matches_oracle(dtype, reader):
     shapes = {f"x{i}": (n,) for i, n in enumerate(SIZES)}
     params = tensors(1, shapes, F32)
     opt = FusedAdamW(params, state_bits=8)
@@ -453,7 +463,7 @@ def test_two_optimizers_on_two_streams():
     assert all(torch.equal(x, y) for x, y in zip(*results))
 
 
-def test_one_gradient_for_two_parameters_and_changed_settings():
+def test_one_gradient_for_two_parameters_and_changed_settings(reader):
     shapes = {"a": (300,), "b": (300,)}
     params = tensors(1, shapes, F32)
     opt = FusedAdamW(params, weight_decay=0.0)
@@ -480,7 +490,7 @@ def test_masters_follow_parameters_when_asked():
     assert torch.equal(opt._views(opt.master_slab)["a"], params["a"].float())
 
 
-def test_inference_tensors():
+def test_inference_tensors(reader):
     with torch.inference_mode():
         g, p = torch.ones(100, device=DEV), torch.zeros(100, device=DEV)
         clip_gradients([g], 1.0)
@@ -490,7 +500,7 @@ def test_inference_tensors():
     assert ((p + 1.0).abs() <= 20 * 2.0 ** -24 + 1e-7).all()
 
 
-def test_replaced_parameter_memory():
+def test_replaced_parameter_memory(reader):
     params = {"a": torch.randn(100, device=DEV), "b": torch.randn(30, device=DEV)}
     opt = FusedAdamW(params)
     ref = Reference(opt, params)
@@ -530,8 +540,43 @@ def test_elements_past_32_bits():
         assert (np.abs(flat(p[s]) - pn) <= bound + 2.0 ** -8 * np.abs(pn)).all()
 
 
+@pytest.mark.parametrize("count", [3, 40])
+def test_native_reader_takes_what_python_takes(count):
+    """The native entries of a clip are those of the checks in Python, and both
+    leave the same calls to a closer look."""
+    import ctypes
+    native = _lib.tensors()
+    back = torch.zeros(100 * count, device=DEV)
+    gl = [back[100 * k:100 * k + 90 + k % 3] for k in range(count)]
+    ol = [torch.zeros(g.shape, dtype=BF16 if k % 2 else F32, device=DEV) for k, g in enumerate(gl)]
+    wide = torch.zeros(2 * gl[-1].numel(), device=DEV)
+    cases = [(gl, gl), (gl, ol), (gl, list(gl)), (gl, gl[1:] + gl[:1]), (gl, ol[:-1] + [ol[0].view(-1)]),
+             (gl[:-1] + [gl[0]], ol), (gl[:-1] + [gl[0]], gl[:-1] + [gl[0]]),
+             (gl, ol[:-1] + [back[50:50 + gl[-1].numel()]]), (gl, ol[:-1] + [wide[::2]]),
+             (gl, ol[:-1] + [wide[:gl[-1].numel()].view(-1, 1)]),
+             (gl[:-1] + [gl[-1].view(BF16)[:9]], gl[:-1] + [gl[-1][:9]])]
+    for k, (g, o) in enumerate(cases):
+        want = _clip_entries(g, o)
+        e, device = np.zeros(count, _ENTRY), ctypes.c_int(-1)
+        version = o[0]._version
+        refused = native.gst_clip(list(g), list(o), e.ctypes.data, count, ctypes.byref(device))
+        assert bool(refused) == (want is None), k
+        if want is not None:
+            # views of one tensor count their changes together
+            assert device.value == 0 and o[0]._version == version + (1 if o is ol else count)
+            for name in ("param", "grad", "n", "cols", "param_stride", "grad_stride", "param_type", "grad_type"):
+                np.testing.assert_array_equal(e[name], want[name], err_msg=f"{k} {name}")
+    e, device = np.zeros(1, _ENTRY), ctypes.c_int(-1)
+    for bad in (torch.zeros(3), torch.zeros(3, device=DEV, dtype=torch.float64), torch.zeros(3, device=DEV).to_sparse(),
+                None, 1.0):
+        assert native.gst_clip([bad], [bad], e.ctypes.data, 1, ctypes.byref(device))
+        assert native.gst_fill([bad], None, None, [torch.zeros(3, device=DEV)], e.ctypes.data, 1, 0)
+    assert native.gst_fill([torch.zeros(4, device=DEV)], None, None, [torch.zeros(3, device=DEV)], e.ctypes.data, 1, 0)
+    assert native.gst_fill(None, None, [torch.zeros(3, device=DEV)], [torch.zeros(3, device=DEV)], e.ctypes.data, 1, 0)
+
+
 # ---------------------------------------------------------------- refusals with device tensors
-def test_refusals_on_the_device():
+def test_refusals_on_the_device(reader):
     params = {"a": torch.zeros(8, device=DEV), "b": torch.zeros(3, device=DEV)}
     with pytest.raises(ValueError, match="one device"):
         FusedAdamW({"a": params["a"], "b": torch.zeros(3)})
