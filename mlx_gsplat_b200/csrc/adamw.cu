@@ -62,9 +62,13 @@ struct AdamWShared {
 // between the norm and the step; the bias corrections are formed by other warps
 // meanwhile (beta^t = 2^(t log2 beta), in 64 bits).
 __device__ __forceinline__ void adamw_prologue(const AdamWArgs& a, AdamWShared& sh) {
+    const int64_t t = *reinterpret_cast<volatile int64_t*>(a.ctl) + 1;
+    if (threadIdx.x == 32)
+        sh.inv_bc1 = 1.0 / (1.0 - exp2((double)t * a.log2_b1));
+    else if (threadIdx.x == 64)
+        sh.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - exp2((double)t * a.log2_b2)));
     double sq = 0.0;
     if (a.partials) sq = sum_partials(a.partials, a.num_partials);
-    const int64_t t = *reinterpret_cast<volatile int64_t*>(a.ctl) + 1;
     if (threadIdx.x == 0) {
         double scale = a.grad_scale;
         bool skip = false;
@@ -78,10 +82,6 @@ __device__ __forceinline__ void adamw_prologue(const AdamWArgs& a, AdamWShared& 
         sh.gscale = (float)scale;
         sh.lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
         sh.step_word = (uint32_t)t * kDitherStep;
-    } else if (threadIdx.x == 32) {
-        sh.inv_bc1 = 1.0 / (1.0 - exp2((double)t * a.log2_b1));
-    } else if (threadIdx.x == 64) {
-        sh.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - exp2((double)t * a.log2_b2)));
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -237,24 +237,30 @@ __global__ void __launch_bounds__(kMultiThreads, kBits == 32 ? kBlocks32 : kBloc
     Segments<kCap> seg(tab);
     int chunks;
     int64_t i;
-    bool more = seg.next(chunks, i);  // every block has a chunk
+    seg.next(chunks, i);  // every block has a chunk
+    int mine, whole;
+    int64_t block;
+    BlockExponents x;
+    // a segment's start: its exponents, in the first segment on their way during the prologue
+    auto enter = [&]() {
+        const TensorEntry& e = tab.e[seg.tensor];
+        i += threadIdx.x * kPerThread;
+        warp_chunks(e.n, i, chunks, mine, whole);
+        block = (e.state + i) / GS_MOMENT_BLOCK;
+        if (kBits == 8) x.load(a.m_exp, a.v_exp, block, kChunk / GS_MOMENT_BLOCK, mine);
+    };
+    enter();
     adamw_prologue(a, sh);
     if (sh.skip) return;
     AdamWTensor t;
     t.gscale = sh.gscale;
     t.inv_sqrt_bc2 = sh.inv_sqrt_bc2;
     t.step_word = sh.step_word;
-    for (; more; more = seg.next(chunks, i)) {
+    for (;;) {
         const TensorEntry& e = tab.e[seg.tensor];
         const double lr = sh.lr * e.lr_scale;
         t.step = (float)(lr * sh.inv_bc1);
         t.keep = (float)(1.0 - lr * e.decay);
-        i += threadIdx.x * kPerThread;
-        int mine, whole;
-        warp_chunks(e.n, i, chunks, mine, whole);
-        const int64_t block = (e.state + i) / GS_MOMENT_BLOCK;
-        BlockExponents x;
-        if (kBits == 8) x.load(a.m_exp, a.v_exp, block, kChunk / GS_MOMENT_BLOCK, mine);
         const bool masters = a.master != nullptr && e.param_type != GS_F32;
         int done = 0;
         if (e.param_vec && e.grad_vec) {
@@ -284,6 +290,8 @@ __global__ void __launch_bounds__(kMultiThreads, kBits == 32 ? kBlocks32 : kBloc
             if (kBits == 8) x.set(done, both & 255u, both >> 8);
         }
         if (kBits == 8) x.store(a.m_exp, a.v_exp, block, kChunk / GS_MOMENT_BLOCK, mine);
+        if (!seg.next(chunks, i)) break;
+        enter();
     }
 }
 

@@ -191,7 +191,7 @@ extern "C" int64_t gs_grad_norm_max_partials(int64_t count) {
     // at most one wave of blocks for every table of tensors
     if (count <= 0) return 0;
     const int64_t cap = count <= kSmallTable ? kSmallTable : kLargeTable;
-    return (count + cap - 1) / cap * (int64_t)sm_count() * kNormBlocksPerSm;
+    return (count + cap - 1) / cap * std::min((int64_t)sm_count() * kNormBlocksPerSm, (int64_t)kMaxGrid);
 }
 
 extern "C" int gs_grad_norm_partials(const gs_tensor* tensors, int64_t count, double* partials, int64_t capacity,

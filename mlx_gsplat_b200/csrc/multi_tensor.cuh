@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace gs {
@@ -30,19 +32,23 @@ struct TensorEntry {
     int8_t param_vec, grad_vec;  // dense and aligned for accesses to eight elements
 };
 
+// Table sizes: a small one for the handful of tensors of a scene (a 2 KB
+// parameter block), and the largest that fits the parameter space with room for
+// a kernel's other arguments.
+constexpr int kSmallTable = 24;
+constexpr int kLargeTable = 360;
+constexpr int kMaxGrid = 640;  // four blocks on each of 160 SMs
+
 template <int kCap>
 struct TensorTable {
     TensorEntry e[kCap];
     int32_t first[kCap + 1];
     int32_t count;
     int32_t group, groups;  // chunks that a block takes at a time, and how many such groups there are
+    // The tensor that each block begins in: a search through a large table costs a block several dependent reads of
+    // parameters that no one has read yet.  (A small table is searched.)
+    uint16_t begin[kCap > kSmallTable ? kMaxGrid : 1];
 };
-
-// Table sizes: a small one for the handful of tensors of a scene (a 2 KB
-// parameter block), and the largest that fits the parameter space with room for
-// a kernel's other arguments.
-constexpr int kSmallTable = 24;
-constexpr int kLargeTable = 368;
 
 // ---------------------------------------------------------------- device side
 // Eight consecutive elements as they lie in memory: 32 bytes of float32 or 16.
@@ -274,6 +280,10 @@ struct Segments {
     __device__ __forceinline__ explicit Segments(const TensorTable<kCap>& t) : tab(t) {
         group = blockIdx.x;  // the grid has at most one block per group
         enter();
+        if (kCap > kSmallTable) {
+            tensor = tab.begin[blockIdx.x];
+            return;
+        }
         int lo = 0, hi = tab.count - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -419,11 +429,19 @@ inline int64_t live_tensors(const gs_tensor* t, int64_t count) {
 template <int kCap>
 inline int table_grid(TensorTable<kCap>& tab, int blocks_per_sm, int most_group) {
     const int64_t chunks = tab.first[tab.count];
-    const int64_t wave = (int64_t)sm_count() * blocks_per_sm;
+    const int64_t wave = std::min((int64_t)sm_count() * blocks_per_sm, (int64_t)kMaxGrid);
     const int64_t rounds = (chunks + wave * most_group - 1) / (wave * most_group);
     tab.group = (int32_t)((chunks + wave * rounds - 1) / (wave * rounds));
     tab.groups = (int32_t)((chunks + tab.group - 1) / tab.group);
-    return (int)(tab.groups < wave ? tab.groups : wave);
+    const int grid = (int)(tab.groups < wave ? tab.groups : wave);
+    if (kCap > kSmallTable) {
+        int t = 0;
+        for (int b = 0; b < grid; ++b) {
+            while (tab.first[t + 1] <= b * tab.group) ++t;
+            tab.begin[b] = (uint16_t)t;
+        }
+    }
+    return grid;
 }
 
 // Launch with programmatic stream serialisation (the kernel begins with
