@@ -459,7 +459,7 @@ class FusedAdamW:
             raise ValueError(f"the step count must not be negative: {t}")
         ml, vl = list(map(m.__getitem__, self.names)), list(map(v.__getitem__, self.names))
         with _on_device(self.device):
-            entries = self._entries.copy()
+            entries = self._entries.view(np.uint8).copy().view(_ENTRY)  # (a copy of bytes: field by field it takes 7 us)
             entries["cols"] = entries["param_stride"] = np.maximum(entries["n"], 1)
             # a tensor's first place takes its m, the second its v
             ml = self._fill_dense(entries, ml, "moment m")

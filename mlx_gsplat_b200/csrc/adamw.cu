@@ -31,9 +31,16 @@ namespace gs {
 // with three), and single chunks keep the blocks closest together (272 us with 16).  8-bit moments:
 // nearly as much arithmetic as memory time, so the registers' most, three; groups
 // as large as the exponents' (moments8.cuh) and no larger.
-constexpr int kBlocks32 = 2, kGroup32 = 1;
-constexpr int kBlocks8 = 3, kGroup8 = 16;
-constexpr int kBlocksQuantize = 4;
+// Where a tensor of the call has rows or odd alignment, its single accesses wait
+// longer and one more block per SM is better (columns of a pool of 1M Gaussians: 481
+// us with three, 516 with two; 8-bit moments 414 with four, 443 with three), which is
+// why such calls have kernels of their own.
+constexpr int kBlocks32 = 2, kBlocks32Rows = 3, kGroup32 = 1;
+constexpr int kBlocks8 = 3, kBlocks8Rows = 4, kGroup8 = 16;
+constexpr int kBlocksQuantize = 4, kBlocksQuantizeRows = 3;
+constexpr int blocks_for(int bits, bool rows) {
+    return bits == 32 ? (rows ? kBlocks32Rows : kBlocks32) : (rows ? kBlocks8Rows : kBlocks8);
+}
 static_assert(kGroup8 <= kSegment, "a warp holds the exponents of a group");
 
 struct AdamWArgs {
@@ -197,18 +204,31 @@ __device__ __forceinline__ void adamw_chunks(const TensorEntry& e, const AdamWAr
 
 // One warp's block of a chunk, where the tensor's end, strides or alignment ask for
 // single accesses.  ``em``, ``ev``: the block's exponents; returns the new ones, v's
-// in the second byte.
-template <int kBits>
+// in the second byte.  kRows: rows or odd alignment may occur.
+template <int kBits, bool kRows>
 __device__ __forceinline__ uint32_t adamw_ragged(const TensorEntry& e, const AdamWArgs& a, const AdamWTensor& t,
                                                  int64_t i, uint32_t em, uint32_t ev) {
     const int64_t s = e.state + i;
     const bool masters = a.master != nullptr && e.param_type != GS_F32;
     float p[8], g[8], m[8], v[8];
-    load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, e.grad_vec, g);
-    if (masters)
-        unpack8(load_raw8(a.master, s, GS_F32), GS_F32, p);
-    else
-        load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, p);
+    if (kRows && !e.grad_vec && !e.param_vec && !masters) {
+        float yg[8], yp[8];
+        start_rows8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, yg);
+        start_rows8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, yp);
+        finish_rows8(yg, g);
+        finish_rows8(yp, p);
+    } else {
+        if (kRows)
+            load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, e.grad_vec, g);
+        else
+            load_tail8(e.grad, i, e.n, e.grad_type, g);
+        if (masters)
+            unpack8(load_raw8(a.master, s, GS_F32), GS_F32, p);
+        else if (kRows)
+            load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, p);
+        else
+            load_tail8(e.param, i, e.n, e.param_type, p);
+    }
     if (kBits == 32) {
         unpack8(load_raw8(a.m, s, GS_F32), GS_F32, m);
         unpack8(load_raw8(a.v, s, GS_F32), GS_F32, v);
@@ -218,7 +238,10 @@ __device__ __forceinline__ uint32_t adamw_ragged(const TensorEntry& e, const Ada
     }
     update8(p, g, m, v, t, a);
     if (masters) store_vec8(a.master, s, GS_F32, p);
-    store_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, p);
+    if (kRows)
+        store_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, p);
+    else
+        store_tail8(e.param, i, e.n, e.param_type, p);
     if (kBits == 32) {
         store_vec8(a.m, s, GS_F32, m);
         store_vec8(a.v, s, GS_F32, v);
@@ -229,8 +252,8 @@ __device__ __forceinline__ uint32_t adamw_ragged(const TensorEntry& e, const Ada
     return em | ev << 8;
 }
 
-template <int kBits, int kCap>
-__global__ void __launch_bounds__(kMultiThreads, kBits == 32 ? kBlocks32 : kBlocks8) adamw_kernel(
+template <int kBits, int kCap, bool kRows>
+__global__ void __launch_bounds__(kMultiThreads, blocks_for(kBits, kRows)) adamw_kernel(
     const __grid_constant__ TensorTable<kCap> tab, const __grid_constant__ AdamWArgs a) {
     __shared__ AdamWShared sh;
     pdl_wait();
@@ -263,7 +286,7 @@ __global__ void __launch_bounds__(kMultiThreads, kBits == 32 ? kBlocks32 : kBloc
         t.keep = (float)(1.0 - lr * e.decay);
         const bool masters = a.master != nullptr && e.param_type != GS_F32;
         int done = 0;
-        if (e.param_vec && e.grad_vec) {
+        if (!kRows || (e.param_vec && e.grad_vec)) {
             done = whole;
             const bool wide_g = e.grad_type == GS_F32;
             if (e.param_type == GS_F32) {
@@ -286,7 +309,7 @@ __global__ void __launch_bounds__(kMultiThreads, kBits == 32 ? kBlocks32 : kBloc
         for (; done < mine; ++done) {
             const uint32_t em = kBits == 8 ? __shfl_sync(kFull, x.m, done) : 0;
             const uint32_t ev = kBits == 8 ? __shfl_sync(kFull, x.v, done) : 0;
-            const uint32_t both = adamw_ragged<kBits>(e, a, t, i + (int64_t)done * kChunk, em, ev);
+            const uint32_t both = adamw_ragged<kBits, kRows>(e, a, t, i + (int64_t)done * kChunk, em, ev);
             if (kBits == 8) x.set(done, both & 255u, both >> 8);
         }
         if (kBits == 8) x.store(a.m_exp, a.v_exp, block, kChunk / GS_MOMENT_BLOCK, mine);
@@ -319,11 +342,17 @@ __device__ __forceinline__ void quantize_chunks(const TensorEntry& e, uint8_t* m
     }
 }
 
+template <bool kRows>
 __device__ __forceinline__ uint32_t quantize_ragged(const TensorEntry& e, uint8_t* mc, uint8_t* vc, int64_t i,
-                                                 uint32_t step_word) {
+                                                    uint32_t step_word) {
     float m[8], v[8];
-    load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, m);
-    load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, e.grad_vec, v);
+    if (kRows) {
+        load_each8(e.param, i, e.n, e.cols, e.param_stride, e.param_type, e.param_vec, m);
+        load_each8(e.grad, i, e.n, e.cols, e.grad_stride, e.grad_type, e.grad_vec, v);
+    } else {
+        load_tail8(e.param, i, e.n, e.param_type, m);
+        load_tail8(e.grad, i, e.n, e.grad_type, v);
+    }
     uint32_t em, ev;
     store_moments8<true>(m, v, (uint32_t)i, step_word, mc + e.state + i, vc + e.state + i, em, ev);
     return em | ev << 8;
@@ -331,8 +360,8 @@ __device__ __forceinline__ uint32_t quantize_ragged(const TensorEntry& e, uint8_
 
 // m (the entries' param) and v (their grad) of any type -> the 8-bit form, with
 // step t's offsets.
-template <int kCap>
-__global__ void __launch_bounds__(kMultiThreads, kBlocksQuantize) moments8_quantize_kernel(
+template <int kCap, bool kRows>
+__global__ void __launch_bounds__(kMultiThreads, kRows ? kBlocksQuantizeRows : kBlocksQuantize) moments8_quantize_kernel(
     const __grid_constant__ TensorTable<kCap> tab, uint8_t* mc, uint8_t* vc, uint8_t* me, uint8_t* ve,
     uint32_t step_word) {
     pdl_wait();
@@ -347,12 +376,12 @@ __global__ void __launch_bounds__(kMultiThreads, kBlocksQuantize) moments8_quant
         const int64_t block = (e.state + i) / GS_MOMENT_BLOCK;
         BlockExponents x;
         int done = 0;
-        if (e.param_vec && e.grad_vec && e.param_type == GS_F32 && e.grad_type == GS_F32) {
+        if ((!kRows || (e.param_vec && e.grad_vec)) && e.param_type == GS_F32 && e.grad_type == GS_F32) {
             quantize_chunks(e, mc, vc, i, whole, step_word, x);
             done = whole;
         }
         for (; done < mine; ++done) {
-            const uint32_t both = quantize_ragged(e, mc, vc, i + (int64_t)done * kChunk, step_word);
+            const uint32_t both = quantize_ragged<kRows>(e, mc, vc, i + (int64_t)done * kChunk, step_word);
             x.set(done, both & 255u, both >> 8);
         }
         x.store(me, ve, block, kChunk / GS_MOMENT_BLOCK, mine);
@@ -379,6 +408,11 @@ __global__ void __launch_bounds__(kMultiThreads) moments8_dequantize_kernel(cons
     store_vec8(v_out, i, kType, x);
 }
 
+template <int kBits, int kCap>
+static const void* adamw_kernel_for(bool all_vec) {
+    return all_vec ? (const void*)adamw_kernel<kBits, kCap, false> : (const void*)adamw_kernel<kBits, kCap, true>;
+}
+
 template <int kCap>
 static int adamw_launches(const gs_tensor* t, int64_t count, int bits, AdamWArgs a, cudaStream_t stream) {
     TensorTable<kCap> tab;
@@ -388,8 +422,8 @@ static int adamw_launches(const gs_tensor* t, int64_t count, int bits, AdamWArgs
         left -= tab.count;
         a.advance = left == 0;
         void* args[] = {&tab, &a};
-        const void* k = bits == 32 ? (const void*)adamw_kernel<32, kCap> : (const void*)adamw_kernel<8, kCap>;
-        const int grid = bits == 32 ? table_grid(tab, kBlocks32, kGroup32) : table_grid(tab, kBlocks8, kGroup8);
+        const void* k = bits == 32 ? adamw_kernel_for<32, kCap>(tab.all_vec) : adamw_kernel_for<8, kCap>(tab.all_vec);
+        const int grid = table_grid(tab, blocks_for(bits, !tab.all_vec), bits == 32 ? kGroup32 : kGroup8);
         GS_TRY(launch_table("adamw_kernel", k, grid, stream, args));
     }
     return GS_OK;
@@ -404,8 +438,10 @@ static int quantize_launches(const gs_tensor* t, int64_t count, uint8_t* m, uint
         at = fill_table(tab, t, at, count);
         left -= tab.count;
         void* args[] = {&tab, &m, &v, &me, &ve, &step_word};
-        GS_TRY(launch_table("moments8_quantize_kernel", (const void*)moments8_quantize_kernel<kCap>,
-                            table_grid(tab, kBlocksQuantize, kGroup8), stream, args));
+        const void* k = tab.all_vec ? (const void*)moments8_quantize_kernel<kCap, false>
+                                    : (const void*)moments8_quantize_kernel<kCap, true>;
+        const int blocks = tab.all_vec ? kBlocksQuantize : kBlocksQuantizeRows;
+        GS_TRY(launch_table("moments8_quantize_kernel", k, table_grid(tab, blocks, kGroup8), stream, args));
     }
     return GS_OK;
 }

@@ -45,6 +45,7 @@ struct TensorTable {
     int32_t first[kCap + 1];
     int32_t count;
     int32_t group, groups;  // chunks that a block takes at a time, and how many such groups there are
+    int32_t all_vec;        // every tensor of the call is dense and aligned
     // The tensor that each block begins in: a search through a large table costs a block several dependent reads of
     // parameters that no one has read yet.  (A small table is searched.)
     uint16_t begin[kCap > kSmallTable ? kMaxGrid : 1];
@@ -188,25 +189,38 @@ struct RowWalk {
 // Eight consecutive elements a lane of a warp's 256, where rows or alignment rule
 // wide accesses out: the warp loads and stores 32 neighbours at a time and turns
 // them round in shared memory.  Every lane takes part; ``i`` is the lane's first
-// element.  (Each lane by itself, eight accesses 32 bytes apart: a step over the
-// columns of a pool of 1M Gaussians takes 628 us instead of 560, with 8-bit moments
-// 513 instead of 431.)
+// element.  Loads begin in start_rows8 and are waited for in finish_rows8, so that
+// two tensors' can be under way together.  (Each lane by itself, eight accesses 32
+// bytes apart: a step over the columns of a pool of 1M Gaussians took 628 us, where
+// it now takes 481.)
 __device__ __forceinline__ float* warp_stage() {
     __shared__ __align__(16) float stage[kMultiThreads / 32][32 * kPerThread];
     return stage[threadIdx.x >> 5];
 }
 
-__device__ __forceinline__ void load_rows8(const void* base, int64_t i, int64_t n, int64_t cols, int64_t stride,
-                                           int type, float (&x)[8]) {
-    const int lane = threadIdx.x & 31;
-    const int64_t left = n - (i - lane * (kPerThread - 1));
-    RowWalk w(i - lane * (kPerThread - 1), cols, stride);
-    float y[8];
+template <int kType>
+__device__ __forceinline__ void gather8(const void* base, RowWalk w, int64_t left, float (&y)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        y[k] = 32 * k < left ? load_one(base, w.off, type) : 0.0f;
+        y[k] = 32 * k < left ? load_one(base, w.off, kType) : 0.0f;
         w.next();
     }
+}
+
+__device__ __forceinline__ void start_rows8(const void* base, int64_t i, int64_t n, int64_t cols, int64_t stride,
+                                            int type, float (&y)[8]) {
+    const int64_t first = i - (threadIdx.x & 31) * (kPerThread - 1);
+    const RowWalk w(first, cols, stride);
+    if (type == GS_F32)
+        gather8<GS_F32>(base, w, n - first, y);
+    else if (type == GS_BF16)
+        gather8<GS_BF16>(base, w, n - first, y);
+    else
+        gather8<GS_F16>(base, w, n - first, y);
+}
+
+__device__ __forceinline__ void finish_rows8(const float (&y)[8], float (&x)[8]) {
+    const int lane = threadIdx.x & 31;
     float* s = warp_stage();
     __syncwarp();
 #pragma unroll
@@ -231,22 +245,18 @@ __device__ __forceinline__ void store_rows8(void* base, int64_t i, int64_t n, in
     for (int k = 0; k < 8; k += 4)
         *reinterpret_cast<float4*>(s + kPerThread * lane + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
     __syncwarp();
-    const int64_t left = n - (i - lane * (kPerThread - 1));
-    RowWalk w(i - lane * (kPerThread - 1), cols, stride);
+    const int64_t first = i - lane * (kPerThread - 1);
+    RowWalk w(first, cols, stride);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        if (32 * k < left) store_one(base, w.off, type, s[32 * k + lane]);
+        if (32 * k < n - first) store_one(base, w.off, type, s[32 * k + lane]);
         w.next();
     }
 }
 
-// The same for any tensor: ``vec`` (of the whole tensor) for wide accesses, with
-// single ones at its end.
-__device__ __forceinline__ void load_each8(const void* base, int64_t i, int64_t n, int64_t cols, int64_t stride,
-                                           int type, bool vec, float (&x)[8]) {
-    if (!vec) {
-        load_rows8(base, i, n, cols, stride, type, x);
-    } else if (i + kPerThread <= n) {
+// Dense, aligned tensors: wide accesses, and single ones at the end.
+__device__ __forceinline__ void load_tail8(const void* base, int64_t i, int64_t n, int type, float (&x)[8]) {
+    if (i + kPerThread <= n) {
         unpack8(load_raw8(base, i, type), type, x);
     } else {
 #pragma unroll
@@ -254,11 +264,8 @@ __device__ __forceinline__ void load_each8(const void* base, int64_t i, int64_t 
     }
 }
 
-__device__ __forceinline__ void store_each8(void* base, int64_t i, int64_t n, int64_t cols, int64_t stride, int type,
-                                            bool vec, const float (&x)[8]) {
-    if (!vec) {
-        store_rows8(base, i, n, cols, stride, type, x);
-    } else if (i + kPerThread <= n) {
+__device__ __forceinline__ void store_tail8(void* base, int64_t i, int64_t n, int type, const float (&x)[8]) {
+    if (i + kPerThread <= n) {
         store_vec8(base, i, type, x);
     } else {
 #pragma unroll
@@ -266,6 +273,26 @@ __device__ __forceinline__ void store_each8(void* base, int64_t i, int64_t n, in
             if (i + k < n) store_one(base, i + k, type, x[k]);
         }
     }
+}
+
+// Any tensor.
+__device__ __forceinline__ void load_each8(const void* base, int64_t i, int64_t n, int64_t cols, int64_t stride,
+                                           int type, bool vec, float (&x)[8]) {
+    if (vec) {
+        load_tail8(base, i, n, type, x);
+    } else {
+        float y[8];
+        start_rows8(base, i, n, cols, stride, type, y);
+        finish_rows8(y, x);
+    }
+}
+
+__device__ __forceinline__ void store_each8(void* base, int64_t i, int64_t n, int64_t cols, int64_t stride, int type,
+                                            bool vec, const float (&x)[8]) {
+    if (vec)
+        store_tail8(base, i, n, type, x);
+    else
+        store_rows8(base, i, n, cols, stride, type, x);
 }
 
 // A block's way through the chunks: it takes every gridDim-th group of successive
@@ -389,6 +416,7 @@ template <int kCap>
 inline int64_t fill_table(TensorTable<kCap>& tab, const gs_tensor* t, int64_t at, int64_t count) {
     int k = 0;
     int64_t chunks = 0;
+    tab.all_vec = 1;
     for (; at < count && k < kCap; ++at) {
         const gs_tensor& s = t[at];
         if (s.n == 0) continue;
@@ -408,6 +436,7 @@ inline int64_t fill_table(TensorTable<kCap>& tab, const gs_tensor* t, int64_t at
         e.grad_type = (int16_t)s.grad_type;
         e.param_vec = can_vector(s.param, s.n, s.cols, s.param_stride);
         e.grad_vec = can_vector(s.grad, s.n, s.cols, s.grad_stride);
+        tab.all_vec &= e.param_vec & e.grad_vec;
         tab.first[k] = (int32_t)chunks;
         chunks += c;
         ++k;
