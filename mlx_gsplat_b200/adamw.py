@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from collections.abc import Mapping
 from functools import partial
 from operator import attrgetter, is_
 from typing import Dict, List, Optional, Sequence, Tuple, Union
@@ -370,6 +371,9 @@ class FusedAdamW:
         norm of the scaled gradients before clipping as a device scalar when
         ``max_norm`` or ``skip_nonfinite`` asks for it, else None."""
         lib = _lib.lib()
+        if grads is not None and not isinstance(grads, Mapping):
+            raise TypeError(f"gradients are given by name, not as {type(grads).__name__}")
+        grad_scale = float(grad_scale)
         if not math.isfinite(grad_scale):
             raise ValueError(f"grad_scale must be finite: {grad_scale}")
         lr, lr_device = self._lr_value()

@@ -12,9 +12,9 @@
 // bits and rounded once.
 //
 // A step moves 28 bytes a float32 parameter with 32-bit moments and 16 with 8-bit
-// ones.  59M parameters (of measured copy rate, 6.55 TB/s): 257 us (98 %) and 154 us
+// ones.  59M parameters (of measured copy rate, 6.55 TB/s): 256 us (98 %) and 153 us
 // (94 %); with 8-bit moments the 53 instructions an element take 60 % of the issue
-// slots, so both bounds are near.  Quantizing them takes 96 us (93 %), reading them
+// slots, so both bounds are near.  Quantizing them takes 97 us (93 %), reading them
 // back as bfloat16 56 us (96 %).
 #include <float.h>
 #include <math.h>

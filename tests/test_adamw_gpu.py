@@ -600,6 +600,10 @@ def test_refusals_on_the_device(reader):
         opt.step({**g, "b": g["b"].to_sparse()})
     with pytest.raises(ValueError, match="no parameter named"):
         opt.step({"z": g["a"]})
+    with pytest.raises(ValueError, match="no parameter named"):
+        opt.step({"a": g["a"], "z": g["b"]})
+    with pytest.raises(TypeError, match="by name"):
+        opt.step(list(g.values()))
     with pytest.raises(ValueError, match="grad_scale"):
         opt.step(g, grad_scale=math.inf)
     with pytest.raises(ValueError, match="exactly"):
