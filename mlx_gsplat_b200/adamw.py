@@ -43,8 +43,6 @@ _is_contiguous = torch.Tensor.is_contiguous
 _device_index = torch.Tensor.get_device
 _dtype = attrgetter("dtype")
 _shape = attrgetter("shape")
-_numel = torch.Tensor.numel
-_same_size = torch.Tensor.is_same_size
 _is_none = partial(is_, None)
 
 
@@ -567,25 +565,23 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
         raise ValueError("no gradients")
     if out is None:
         ol = gl
-    entries, index = np.zeros(len(gl), _ENTRY), ctypes.c_int(-1)
+    n = len(gl)
     native = _lib.tensors()
-    filled = native is not None and not native.gst_clip(gl, ol, entries.ctypes.data, len(gl), ctypes.byref(index))
-    try:
-        entries = entries if filled else _clip_entries(gl, ol)
-    except (KeyError, AttributeError, TypeError, RuntimeError):
-        for name, g, o in zip(names, gl, ol):
-            _check_tensor(f"gradient {name!r}", g)
-            _check_tensor(f"out {name!r}", o)
-        raise
-    if entries is None:
-        entries, gl = _clip_entries_strided(names, gl, ol)
-    device = torch.device("cuda", index.value) if filled else _check_cuda(gl + ol)
+    if native is not None:
+        table, found = (ctypes.c_char * (_ENTRY.itemsize * n))(), (ctypes.c_int * 2)()
+        at = ctypes.addressof(table)
+    filled = native is not None and not native.gst_clip(gl, ol, at, n, found)
+    if filled:
+        device, elements = torch.device("cuda", found[0]), found[1]
+    else:
+        entries, gl = _clip_entries(names, gl, ol)
+        device, elements, at = _check_cuda(gl + ol), entries["n"].any(), entries.ctypes.data
     lib = _lib.lib()
     with _on_device(device):
         norm = torch.empty((), dtype=torch.float32, device=device)
-        if not entries["n"].any():
+        if not elements:
             return norm.zero_()
-        at, n, stream = entries.ctypes.data, len(entries), _lib.stream_ptr(device)
+        stream = _lib.stream_ptr(device)
         partials = torch.empty(lib.gs_grad_norm_max_partials(n), dtype=torch.float64, device=device)
         count = _norm_partials(lib, at, n, partials, stream)
         _lib.check(lib.gs_clip_gradients(at, n, partials.data_ptr(), count, max_norm, norm.data_ptr(), stream),
@@ -595,79 +591,7 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
     return norm
 
 
-# Up to so many tensors, plain loops take less time than array operations (6 tensors: 8 us against 16).
-_FEW = 16
-
-
-def _clip_entries_few(gl: List[torch.Tensor], ol: List[torch.Tensor]) -> Optional[np.ndarray]:
-    apart = ol is not gl
-    words, inputs, outputs = [], [], []
-    for g, o in zip(gl, ol):
-        if not g.is_contiguous():
-            return None
-        n, g_ptr, g_type = g.numel(), g.data_ptr(), TYPES[g.dtype]
-        o_ptr, o_type = g_ptr, g_type
-        if apart:
-            if not (o.is_contiguous() and o.shape == g.shape):
-                return None
-            o_ptr, o_type = o.data_ptr(), TYPES[o.dtype]
-            if o_ptr != g_ptr or o_type != g_type:  # a gradient may lie in its own output's memory
-                inputs.append((g_ptr, g_ptr + n * (2 if g_type else 4)))
-        outputs.append((o_ptr, o_ptr + n * (2 if o_type else 4)))
-        d = n or 1
-        words += (o_ptr, g_ptr, n, 0, d, d, d, o_type | g_type << 32, 0, 0)
-    outputs.sort()
-    reach = 0
-    for lo, hi in outputs:
-        if lo < reach:
-            return None
-        reach = hi
-    if inputs and min(inputs)[0] < reach and max(hi for _, hi in inputs) > outputs[0][0]:
-        if any(lo < b and hi > a for lo, hi in inputs for a, b in outputs):
-            return None
-    return np.array(words, np.int64).view(_ENTRY)
-
-
-def _clip_entries(gl: List[torch.Tensor], ol: List[torch.Tensor]) -> Optional[np.ndarray]:
-    """The entries where every tensor is dense and none shares memory that
-    another one writes; None where that takes a closer look."""
-    n = len(gl)
-    if n <= _FEW:
-        return _clip_entries_few(gl, ol)
-    apart = ol is not gl
-    every = gl + ol if apart else gl
-    if not all(map(_is_contiguous, every)) or (apart and not all(map(_same_size, gl, ol))):
-        return None
-    types = list(map(_dtype, every))
-    if types.count(types[0]) == len(types):
-        g_type = o_type = TYPES[types[0]]
-    else:
-        codes = np.array([TYPES[t] for t in types], np.int64)
-        g_type, o_type = codes[:n], codes[-n:]
-    ptr = np.array(list(map(_data_ptr, every)), np.int64)
-    g_ptr, o_ptr = ptr[:n], ptr[-n:]
-    size = np.array(list(map(_numel, gl)), np.int64)
-    words = np.zeros((n, _ENTRY.itemsize // 8), np.int64)  # the entries' fields, the two types sharing a word
-    words[:, 0], words[:, 1], words[:, 2] = o_ptr, g_ptr, size
-    words[:, 4:7] = np.maximum(size, 1)[:, None]
-    words[:, 7] = o_type + g_type * (1 << 32)
-    if n > 1 or apart:
-        o_end = o_ptr + size * (4 - 2 * (o_type != _lib.GS_F32))
-        order = o_ptr.argsort()
-        starts, ends = o_ptr[order], o_end[order]
-        if (ends[:-1] > starts[1:]).any():
-            return None
-    if apart:
-        # a gradient may lie in its own output's memory, or in none: the last output that starts below its end
-        g_end = g_ptr + size * (4 - 2 * (g_type != _lib.GS_F32))
-        last = starts.searchsorted(g_end) - 1
-        shared = (ends[last] > g_ptr) & (last >= 0)
-        if shared.any() and (shared & ((g_ptr != o_ptr) | (g_type != o_type))).any():
-            return None
-    return words.view(_ENTRY).reshape(n)
-
-
-def _clip_entries_strided(names, gl: List[torch.Tensor], ol: List[torch.Tensor]):
+def _clip_entries(names, gl: List[torch.Tensor], ol: List[torch.Tensor]) -> Tuple[np.ndarray, List[torch.Tensor]]:
     """The entries of any tensors, with the refusals; and the gradients, dense
     copies in the place of those that are not rows."""
     in_place = ol is gl

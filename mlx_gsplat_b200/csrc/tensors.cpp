@@ -96,23 +96,25 @@ extern "C" int gst_params_unmoved(PyObject* params, const gs_tensor* e, Py_ssize
 // The entries of gradients and of the tensors their clipped values go to (the same
 // list: in place), where all are dense and on one device (returned) and nothing
 // that is written overlaps anything but its own gradient's memory.  ``e`` comes
-// zeroed.
-extern "C" int gst_clip(PyObject* grads, PyObject* outs, gs_tensor* e, Py_ssize_t n, int* device) {
+// zeroed; ``found``: the device, and whether there is any element.
+extern "C" int gst_clip(PyObject* grads, PyObject* outs, gs_tensor* e, Py_ssize_t n, int* found) {
     try {
         if (!PyList_Check(grads) || !PyList_Check(outs) || PyList_GET_SIZE(grads) != n || PyList_GET_SIZE(outs) != n || n == 0)
             return 1;
         const at::Tensor* first = tensor_of(PyList_GET_ITEM(grads, 0));
         if (!first || !first->defined() || !first->is_cuda()) return 1;
-        *device = first->get_device();
+        const int device = first->get_device();
+        bool any = false;
         std::vector<Span> written(n), read;
         for (Py_ssize_t k = 0; k < n; ++k) {
             const at::Tensor* g = tensor_of(PyList_GET_ITEM(grads, k));
             const at::Tensor* o = tensor_of(PyList_GET_ITEM(outs, k));
             if (!g || !o) return 1;
-            const int g_type = dense_type(*g, *device), o_type = dense_type(*o, *device);
+            const int g_type = dense_type(*g, device), o_type = dense_type(*o, device);
             if (g_type < 0 || o_type < 0 || g->sizes() != o->sizes()) return 1;
             gs_tensor& t = e[k];
             t.n = g->numel();
+            any |= t.n > 0;
             t.param = o->mutable_data_ptr();
             t.grad = g->const_data_ptr();
             t.param_type = o_type;
@@ -131,6 +133,8 @@ extern "C" int gst_clip(PyObject* grads, PyObject* outs, gs_tensor* e, Py_ssize_
             if (w != written.begin() && (w - 1)->hi > r.lo) return 1;
         }
         for (Py_ssize_t k = 0; k < n; ++k) changed(*tensor_of(PyList_GET_ITEM(outs, k)));
+        found[0] = device;
+        found[1] = any;
         return 0;
     } catch (...) {
         return 1;

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from mlx_gsplat_b200 import FusedAdamW, _lib, clip_gradients
-from mlx_gsplat_b200.adamw import _ENTRY, overlapping, rows_of
+from mlx_gsplat_b200.adamw import _ENTRY, _clip_entries, overlapping, rows_of
 from oracle import adamw as oadamw
 
 built = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
@@ -118,33 +118,40 @@ def test_bad_clipping():
         clip_gradients([big[:8]], 1.0, out=[big[:8]])
 
 
-@pytest.mark.parametrize("count", [3, 16, 17, 40])  # plain loops, array operations
-def test_entries_of_dense_tensors(count):
-    """The dense tensors' entries, and the cases that take a closer look."""
-    from mlx_gsplat_b200.adamw import _clip_entries
-    back = torch.zeros(100 * count)
+def clip_cases(count, device):
+    """(gradients, outputs, whether dense and apart, whether refused)"""
+    back = torch.zeros(100 * count, device=device)
     gl = [back[100 * k:100 * k + 90 + k % 3] for k in range(count)]
-    ol = [torch.zeros(g.shape, dtype=torch.bfloat16 if k % 2 else torch.float32) for k, g in enumerate(gl)]
-    for out in (gl, ol):
-        e = _clip_entries(gl, out)
-        assert e["grad"].tolist() == [g.data_ptr() for g in gl] and e["param"].tolist() == [o.data_ptr() for o in out]
-        for name in ("n", "cols", "param_stride", "grad_stride"):
-            assert e[name].tolist() == [g.numel() for g in gl]
+    ol = [torch.zeros(g.shape, dtype=torch.bfloat16 if k % 2 else torch.float32, device=device)
+          for k, g in enumerate(gl)]
+    wide = torch.zeros(2 * gl[-1].numel(), device=device)
+    last = gl[-1].numel()
+    return [(gl, gl, True, False), (gl, ol, True, False), (gl, list(gl), True, False),
+            (gl[:-1] + [gl[0]], ol[:-1] + [ol[-1].new_zeros(gl[0].shape)], True, False),  # read twice
+            (gl, ol[:-1] + [wide[::2]], False, False),                                     # strided
+            (gl, gl[1:] + gl[:1], False, True),                                            # in others' memory
+            (gl, [ol[-1][:gl[0].numel()]] + ol[1:], False, True),                          # written twice
+            (gl[:-1] + [gl[0]], gl[:-1] + [gl[0]], False, True),
+            (gl, ol[:-1] + [back[50:50 + last]], False, True),                             # part of another gradient
+            (gl, ol[:-1] + [wide[:last].view(-1, 1)], False, True),                        # another shape
+            (gl[:-1] + [gl[-1].view(torch.bfloat16)[:9]], gl[:-1] + [gl[-1][:9]], False, True)]  # another type
+
+
+@pytest.mark.parametrize("count", [3, 40])
+def test_entries_of_clipping(count):
+    for k, (gl, ol, dense, refused) in enumerate(clip_cases(count, "cpu")):
+        if refused:
+            with pytest.raises(ValueError, match="shape|share|another"):
+                _clip_entries(range(count), gl, ol)
+            continue
+        e, kept = _clip_entries(range(count), gl, ol)
+        assert e["grad"].tolist() == [g.data_ptr() for g in kept] and e["param"].tolist() == [o.data_ptr() for o in ol]
+        assert e["n"].tolist() == [g.numel() for g in gl]
+        if dense:
+            for name in ("cols", "param_stride", "grad_stride"):
+                assert e[name].tolist() == [g.numel() for g in gl]
         assert e["grad_type"].tolist() == [0] * count
-        assert e["param_type"].tolist() == [int(o.dtype == torch.bfloat16) for o in out]
-    same = list(gl)
-    assert _clip_entries(gl, same) is not None  # each in its own memory
-    assert _clip_entries(gl, same[1:] + same[:1]) is None  # in others'
-    assert _clip_entries(gl, ol[:-1] + [ol[0].view(-1)]) is None  # written twice
-    assert _clip_entries(gl[:-1] + [gl[0]], gl[:-1] + [gl[0]]) is None
-    assert _clip_entries(gl, ol[:-1] + [back[100 * count - 50:].new_zeros(gl[-1].shape)]) is not None
-    assert _clip_entries(gl, ol[:-1] + [back[50:50 + gl[-1].numel()]]) is None  # part of another gradient
-    assert _clip_entries(gl, ol[:-1] + [torch.zeros(2 * gl[-1].numel())[::2]]) is None  # strided
-    assert _clip_entries(gl, ol[:-1] + [torch.zeros(gl[-1].numel(), 1)]) is None  # another shape
-    assert _clip_entries(gl[:-1] + [gl[-1].view(torch.bfloat16)[:9]], gl[:-1] + [gl[-1][:9]]) is None  # another type
-    zero = [torch.zeros(0)] * count
-    e = _clip_entries(zero, zero)
-    assert e is None or not e["n"].any()
+        assert e["param_type"].tolist() == [int(o.dtype == torch.bfloat16) for o in ol]
 
 
 def test_calls_are_made_on_the_tensors_device(monkeypatch):
@@ -231,11 +238,11 @@ def test_native_reader_leaves_host_tensors_alone():
     native = _lib.tensors()
     if native is None:
         pytest.skip("helper not built")
-    e, device, t = np.zeros(1, _ENTRY), ctypes.c_int(-1), torch.zeros(3)
+    e, device, t = np.zeros(1, _ENTRY), (ctypes.c_int * 2)(-1, -1), torch.zeros(3)
     for items in ([t], {"a": t}, None, (t,), [t, t], 3):
         assert native.gst_fill(items, ["a"], [t], [t], e.ctypes.data, 1, 0) == 1
-    assert native.gst_clip([t], [t], e.ctypes.data, 1, ctypes.byref(device)) == 1
-    assert native.gst_clip([], [], e.ctypes.data, 0, ctypes.byref(device)) == 1
+    assert native.gst_clip([t], [t], e.ctypes.data, 1, device) == 1
+    assert native.gst_clip([], [], e.ctypes.data, 0, device) == 1
     assert native.gst_params_unmoved([t], e.ctypes.data, 1) == 1 and t._version == 0
     e["param"] = t.data_ptr()
     assert native.gst_params_unmoved([t], e.ctypes.data, 1) == 0 and t._version == 1

@@ -108,6 +108,24 @@ def test_step_matches_oracle(bits, ptype, gtype, master):
                   master=master)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("scale,betas,eps", [(1e-24, (0.9, 0.999), 1e-8), (1e-12, (0.9, 0.999), 1e-15),
+                                             (1e15, (0.9, 0.999), 1e-8), (1.0, (0.0, 0.0), 1e-8),
+                                             (1.0, (0.0, 0.99), 1e-3), (1.0, (0.95, 0.0), 1e-8)])
+def test_gradient_sizes_and_betas(bits, scale, betas, eps):
+    """Squares past float32's normal range on both sides, and corrections of betas
+    of 0.  (A root of a float32 v that underflows is off by 2^-74 at most, against
+    an eps of 1e-8 nothing.)"""
+    shapes = {"a": (5000,), "b": (300,)}
+    params = tensors(1, shapes, F32)
+    opt = FusedAdamW(params, lr=1e-2, betas=betas, eps=eps, state_bits=bits, weight_decay=0.3)
+    ref = Reference(opt, params)
+    for s in range(3):
+        grads = tensors(10 + s, shapes, F32, scale=scale)
+        opt.step(grads)
+        ref.check(grads, lr=1e-2)
+
+
 def test_mixed_types_in_one_step_and_grad_scale(reader):
     shapes = {"a": (33, 5), "b": (2050,), "c": (7, 11, 13), "d": ()}
     params = {**tensors(1, {"a": shapes["a"], "d": ()}, F32), **tensors(2, {"b": shapes["b"]}, BF16),
@@ -541,35 +559,29 @@ def test_elements_past_32_bits():
 
 
 @pytest.mark.parametrize("count", [3, 40])
-def test_native_reader_takes_what_python_takes(count):
-    """The native entries of a clip are those of the checks in Python, and both
-    leave the same calls to a closer look."""
+def test_native_reader_takes_dense_tensors_only(count):
+    """The native entries of a clip are those of the checks in Python; strided and
+    refused calls are left to these."""
     import ctypes
+
+    from test_adamw import clip_cases
     native = _lib.tensors()
-    back = torch.zeros(100 * count, device=DEV)
-    gl = [back[100 * k:100 * k + 90 + k % 3] for k in range(count)]
-    ol = [torch.zeros(g.shape, dtype=BF16 if k % 2 else F32, device=DEV) for k, g in enumerate(gl)]
-    wide = torch.zeros(2 * gl[-1].numel(), device=DEV)
-    cases = [(gl, gl), (gl, ol), (gl, list(gl)), (gl, gl[1:] + gl[:1]), (gl, ol[:-1] + [ol[0].view(-1)]),
-             (gl[:-1] + [gl[0]], ol), (gl[:-1] + [gl[0]], gl[:-1] + [gl[0]]),
-             (gl, ol[:-1] + [back[50:50 + gl[-1].numel()]]), (gl, ol[:-1] + [wide[::2]]),
-             (gl, ol[:-1] + [wide[:gl[-1].numel()].view(-1, 1)]),
-             (gl[:-1] + [gl[-1].view(BF16)[:9]], gl[:-1] + [gl[-1][:9]])]
-    for k, (g, o) in enumerate(cases):
-        want = _clip_entries(g, o)
-        e, device = np.zeros(count, _ENTRY), ctypes.c_int(-1)
-        version = o[0]._version
-        refused = native.gst_clip(list(g), list(o), e.ctypes.data, count, ctypes.byref(device))
-        assert bool(refused) == (want is None), k
-        if want is not None:
-            # views of one tensor count their changes together
-            assert device.value == 0 and o[0]._version == version + (1 if o is ol else count)
+    for k, (g, o, dense, _) in enumerate(clip_cases(count, DEV)):
+        e, device = np.zeros(count, _ENTRY), (ctypes.c_int * 2)(-1, -1)
+        before = sum(x._version for x in o)
+        refused = native.gst_clip(list(g), list(o), e.ctypes.data, count, device)
+        assert bool(refused) == (not dense), k
+        if dense:
+            assert list(device) == [0, 1] and sum(x._version for x in o) > before
+            want, _ = _clip_entries(range(count), g, o)
             for name in ("param", "grad", "n", "cols", "param_stride", "grad_stride", "param_type", "grad_type"):
                 np.testing.assert_array_equal(e[name], want[name], err_msg=f"{k} {name}")
-    e, device = np.zeros(1, _ENTRY), ctypes.c_int(-1)
+        else:
+            assert sum(x._version for x in o) == before
+    e, device = np.zeros(1, _ENTRY), (ctypes.c_int * 2)(-1, -1)
     for bad in (torch.zeros(3), torch.zeros(3, device=DEV, dtype=torch.float64), torch.zeros(3, device=DEV).to_sparse(),
                 None, 1.0):
-        assert native.gst_clip([bad], [bad], e.ctypes.data, 1, ctypes.byref(device))
+        assert native.gst_clip([bad], [bad], e.ctypes.data, 1, device)
         assert native.gst_fill([bad], None, None, [torch.zeros(3, device=DEV)], e.ctypes.data, 1, 0)
     assert native.gst_fill([torch.zeros(4, device=DEV)], None, None, [torch.zeros(3, device=DEV)], e.ctypes.data, 1, 0)
     assert native.gst_fill(None, None, [torch.zeros(3, device=DEV)], [torch.zeros(3, device=DEV)], e.ctypes.data, 1, 0)
