@@ -250,6 +250,7 @@ class FusedAdamW:
         self.m_exp = torch.zeros(blocks, dtype=torch.uint8, device=self.device)
         self.v_exp = torch.zeros(blocks, dtype=torch.uint8, device=self.device)
         self._control = torch.zeros(2, dtype=torch.int64, device=self.device)
+        self._count = self._control[0]
         self.master_slab: Optional[torch.Tensor] = None
         if master_weights and any(p.dtype != torch.float32 for p in self._params):
             self.master_slab = torch.zeros(self.slab_elements, dtype=torch.float32, device=self.device)
@@ -424,13 +425,13 @@ class FusedAdamW:
     @property
     def t(self) -> int:
         """Steps taken (read from the device: a host sync)."""
-        return int(self._control[0])
+        return int(self._count)
 
     @t.setter
     def t(self, value: int) -> None:
         if value < 0:
             raise ValueError(f"the step count must not be negative: {value}")
-        self._control[0] = int(value)
+        self._count.fill_(int(value))
 
     def _views(self, slab: torch.Tensor) -> Dict[str, torch.Tensor]:
         return {k: slab[self.offsets[k]:self.offsets[k] + s.numel()].view(s)
@@ -470,7 +471,7 @@ class FusedAdamW:
             if t is None:
                 t = self.t if self.state_bits == 8 else None
             else:
-                self._control[0].fill_(int(t))
+                self._count.fill_(int(t))
             if self.state_bits == 32:
                 torch._foreach_copy_(list(self._views(self.m).values()) + list(self._views(self.v).values()), ml + vl)
                 return
