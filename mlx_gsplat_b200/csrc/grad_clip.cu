@@ -4,14 +4,14 @@
 //   g'   = g * max_norm / norm   when norm > max_norm
 //
 // The squares are formed and summed in 64 bits: a norm over tens of millions of
-// elements is then correct to float32's last bit whatever the order, is finite in
-// float32 wherever it lies in float32's range, and the order is fixed (each block writes one
-// partial sum, every consumer adds them in index order), so a run repeats bit for
-// bit.  Finding the norm has to read every gradient before the first may be
-// scaled; only gradients that still lie in the 126 MB L2 are not read from
-// memory twice.  59M float32: norm 36 us (of measured copy rate: 100 %), norm and
-// clipping into other tensors 119 us (three passes: 91 %); bfloat16 is held up by
-// the conversions to 64 bits (norm 22 us, 81 %).
+// elements is then correct to float32's last bit whatever the order, and finite in
+// float32 wherever it lies in float32's range.  The order is fixed too (each block
+// writes one partial sum, every consumer adds them in index order), so a run
+// repeats bit for bit.  Finding the norm has to read every gradient before the
+// first may be scaled; only gradients that still lie in the 126 MB L2 are not read
+// from memory twice.  59M float32: norm 36 us (of measured copy rate: 100 %), norm
+// and clipping into other tensors 119 us (three passes: 91 %); bfloat16 is held up
+// by the conversions to 64 bits (norm 22 us, 81 %).
 #include <math.h>
 
 #include "multi_tensor.cuh"
