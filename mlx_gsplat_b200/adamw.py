@@ -40,6 +40,7 @@ _ENTRY = np.dtype([("param", np.uint64), ("grad", np.uint64), ("n", np.int64), (
                    ("decay", np.float64)], align=True)
 _data_ptr = torch.Tensor.data_ptr
 _is_contiguous = torch.Tensor.is_contiguous
+_is_neg = torch.Tensor.is_neg
 _device_index = torch.Tensor.get_device
 _dtype = attrgetter("dtype")
 _shape = attrgetter("shape")
@@ -108,6 +109,12 @@ def _check_tensor(what: str, t) -> None:
         raise ValueError(f"{what}: sparse tensors are not supported")
     if t.dtype not in TYPES:
         raise ValueError(f"{what}: {t.dtype} is not float32, bfloat16 or float16")
+
+
+def _check_written(what: str, t) -> None:
+    _check_tensor(what, t)
+    if t.is_neg():
+        raise ValueError(f"{what}: a view that reads as the negative of its memory cannot be written")
 
 
 def _check_cuda(tensors: Sequence[torch.Tensor]) -> torch.device:
@@ -206,7 +213,7 @@ class FusedAdamW:
         self._params = [params[k] for k in self.names]
         self._rows = []
         for name, p in params.items():
-            _check_tensor(f"parameter {name!r}", p)
+            _check_written(f"parameter {name!r}", p)
             rows = rows_of(p)
             if rows is None:
                 raise ValueError(f"parameter {name!r}: strides {tuple(p.stride())} of shape {tuple(p.shape)} are "
@@ -279,6 +286,8 @@ class FusedAdamW:
         if isinstance(lr, torch.Tensor):
             if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != self.device:
                 raise ValueError("a tensor lr is one float32 on the parameters' device")
+            if lr.is_neg():
+                raise ValueError("a tensor lr may not be a view that reads as the negative of its memory")
             return 0.0, lr.data_ptr()
         lr = float(lr)
         if not (math.isfinite(lr) and lr >= 0.0):
@@ -326,6 +335,8 @@ class FusedAdamW:
         ``shapes``); returns the entries (a copy where their rows had to change)
         and the tensors that must outlive the launch."""
         try:
+            if any(map(_is_neg, grads)):  # views that read as the negative of their memory (autograd makes some)
+                grads = [g.resolve_neg() for g in grads]
             types = list(map(_dtype, grads))
             codes = list(map(TYPES.__getitem__, types)) if types.count(types[0]) != len(types) else TYPES[types[0]]
             same = list(map(_shape, grads)) == shapes
@@ -593,14 +604,15 @@ def clip_gradients(grads: Tensors, max_norm: float, out: Optional[Tensors] = Non
 
 
 def _clip_entries(names, gl: List[torch.Tensor], ol: List[torch.Tensor]) -> Tuple[np.ndarray, List[torch.Tensor]]:
-    """The entries of any tensors, with the refusals; and the gradients, dense
-    copies in the place of those that are not rows."""
+    """The entries of any tensors, with the refusals; and the gradients, copies
+    in the place of those that are not rows or read as the negative of their memory."""
     in_place = ol is gl
     for name, g, o in zip(names, gl, ol):
         _check_tensor(f"gradient {name!r}", g)
-        _check_tensor(f"out {name!r}", o)
+        _check_written(f"{'gradient' if in_place else 'out'} {name!r}", o)
         if o.shape != g.shape:
             raise ValueError(f"out {name!r} has shape {tuple(o.shape)}, not {tuple(g.shape)}")
+    gl = [g.resolve_neg() for g in gl]
     g_rows, o_rows = list(map(rows_of, gl)), list(map(rows_of, ol))
     for name, o, rows in zip(names, ol, o_rows):
         if rows is None:
@@ -610,7 +622,6 @@ def _clip_entries(names, gl: List[torch.Tensor], ol: List[torch.Tensor]) -> Tupl
         raise ValueError("written tensors share memory")
     if not in_place:
         _check_apart(gl, ol, o_rows)
-    gl = list(gl)
     entries = np.zeros(len(gl), _ENTRY)
     for k, (g, o) in enumerate(zip(gl, ol)):
         (o_cols, o_stride), rows = o_rows[k], g_rows[k]

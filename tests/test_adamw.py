@@ -295,3 +295,35 @@ def test_positive_v_stays_positive():
     for t in range(50):
         c, _ = oadamw.quantize(x, t, True)
         assert c[5] == 0 and (np.delete(c, 5) > 0).all()
+
+
+# ---------------------------------------------------------------- views that read as the negative of their memory
+def memory(address, n):
+    return np.ctypeslib.as_array((ctypes.c_float * n).from_address(int(address))).copy()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_negated_gradients_are_resolved(strided):
+    """A gradient with the negation bit (autograd makes them behind ``conj``) is
+    read by its values, not by its memory's; nothing is written through one."""
+    from types import SimpleNamespace
+    if strided:
+        g = torch.view_as_complex(torch.arange(1.0, 9.0).view(4, 2)).conj().imag
+    else:
+        g = torch._neg_view(torch.arange(1.0, 5.0))
+    assert g.is_neg()
+    want = g.clone()
+    host = SimpleNamespace(device=SimpleNamespace(index=-1))  # a host tensor's device index
+    e, kept = FusedAdamW._with_grads(host, _entry(n=4, cols=4, param_stride=4), ["a"], [g.shape], [g])
+    np.testing.assert_array_equal(memory(e["grad"][0], 4), want)
+    assert int(e["grad_stride"][0]) == 4 and torch.equal(kept[0], want)
+    e, kept = _clip_entries(range(2), [g, want], [torch.zeros(4), torch.zeros(4)])
+    np.testing.assert_array_equal(memory(e["grad"][0], 4), want)
+    np.testing.assert_array_equal(memory(e["grad"][1], 4), want)
+    assert torch.equal(kept[0], want)
+    with pytest.raises(ValueError, match="negative"):
+        _clip_entries(range(1), [want], [g])
+    with pytest.raises(ValueError, match="negative"):
+        clip_gradients([g], 1.0)
+    with pytest.raises(ValueError, match="negative"):
+        FusedAdamW({"a": g})

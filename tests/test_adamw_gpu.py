@@ -705,3 +705,56 @@ def test_beside_the_pooled_adam():
             # each side: at most 16 roundings of the step and 2 of the parameter, a step
             tol = (s + 1) * 2.0 ** -24 * (32 * 1e-2 * 8 + 4 * before[k].abs())
             assert ((p[k] - q[k]).abs() <= tol).all()
+
+
+# ---------------------------------------------------------------- views that read as the negative of their memory
+def negated(x, strided):
+    """A tensor of x's values that has the negation bit."""
+    if strided:
+        return torch.view_as_complex(torch.stack([torch.zeros_like(x), -x], -1)).conj().imag
+    return torch._neg_view(-x)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_negated_gradients_and_moments(bits, strided, reader):
+    shapes = {"a": (700,), "b": (33, 3)}
+    plain, other = tensors(1, shapes, F32), tensors(1, shapes, F32)
+    one, two = FusedAdamW(plain, state_bits=bits, max_norm=0.1), FusedAdamW(other, state_bits=bits, max_norm=0.1)
+    m = tensors(2, shapes, F32)
+    v = {k: x.square() for k, x in tensors(3, shapes, F32).items()}
+    one.load_moments(m, v, t=5)
+    two.load_moments({**m, "a": negated(m["a"], strided)}, v, t=5)
+    g = tensors(4, shapes, F32)
+    n = {k: negated(x, strided) for k, x in g.items()}
+    assert n["a"].is_neg() and torch.equal(n["a"], g["a"])
+    one.step(g)
+    two.step({"a": n["a"], "b": g["b"]})
+    one.step(g)
+    two.step(n)
+    assert all(torch.equal(plain[k], other[k]) for k in shapes)
+    assert torch.equal(one.m, two.m) and torch.equal(one.v, two.v)
+    outs = [[torch.zeros_like(x) for x in g.values()] for _ in range(2)]
+    norms = [clip_gradients(list(x.values()), 0.1, out=o) for x, o in zip((g, n), outs)]
+    assert torch.equal(*norms) and all(torch.equal(x, y) for x, y in zip(*outs))
+    with pytest.raises(ValueError, match="negative"):
+        clip_gradients(n, 0.1)
+    with pytest.raises(ValueError, match="negative"):
+        clip_gradients(g, 0.1, out=n)
+    with pytest.raises(ValueError, match="negative"):
+        FusedAdamW(n)
+    two.lr = torch._neg_view(torch.tensor([-0.5], device=DEV))
+    with pytest.raises(ValueError, match="negative"):
+        two.step(g)
+
+
+def test_gradients_that_autograd_negates(reader):
+    a, b = (torch.randn(50, device=DEV, requires_grad=True) for _ in range(2))
+    c = torch.randn(50, dtype=torch.complex64, device=DEV)
+    grads = dict(zip("ab", torch.autograd.grad((torch.complex(a, b).conj() + c).abs().sum(), [a, b])))
+    assert grads["b"].is_neg()
+    params = {"a": a, "b": b}
+    opt = FusedAdamW(params)
+    ref = Reference(opt, params)
+    opt.step(grads)
+    ref.check(grads)
