@@ -44,6 +44,7 @@ _is_neg = torch.Tensor.is_neg
 _device_index = torch.Tensor.get_device
 _dtype = attrgetter("dtype")
 _shape = attrgetter("shape")
+_stride = torch.Tensor.stride
 _is_none = partial(is_, None)
 
 
@@ -231,10 +232,8 @@ class FusedAdamW:
         self.max_norm = max_norm
         self._lr_value()
         self._norm_limit()
-        # aliases keep the memory that the entries point to alive whatever happens to the caller's tensors
-        self._aliases = [p.detach() for p in self._params]
-        self._ptrs = list(map(_data_ptr, self._params))
         self._shapes = list(map(_shape, self._params))
+        self._take_memory()
         n = len(self._params)
         sizes = [p.numel() for p in self._params]
         room = [-(-s // BLOCK) * BLOCK for s in sizes]
@@ -309,21 +308,32 @@ class FusedAdamW:
             self._partials = torch.empty(size, dtype=torch.float64, device=self.device)
         return self._partials
 
+    def _take_memory(self) -> None:
+        # aliases keep the memory that the entries point to alive, and its layout, whatever happens to the caller's tensors
+        self._aliases = [p.detach() for p in self._params]
+        self._ptrs = list(map(_data_ptr, self._params))
+        self._types = list(map(_dtype, self._params))
+        self._strides = list(map(_stride, self._params))
+
+    def _as_taken(self) -> bool:
+        """Whether the parameters are the memory, types and layouts of the entries."""
+        ps = self._params
+        return list(map(_data_ptr, ps)) == self._ptrs and list(map(_dtype, ps)) == self._types and \
+            list(map(_shape, ps)) == self._shapes and list(map(_stride, ps)) == self._strides and \
+            not any(map(_is_neg, ps))
+
     def _refresh(self) -> None:
         """The parameters' memory was replaced (``p.data = ...``): takes the new
         memory when it has the old form."""
         for k, (name, p) in enumerate(zip(self.names, self._params)):
-            if p.data_ptr() == self._ptrs[k]:
-                continue
-            if p.dtype != self._aliases[k].dtype or p.shape != self._shapes[k] or p.device != self.device or \
-                    rows_of(p) != self._rows[k]:
+            if p.layout != torch.strided or p.dtype != self._types[k] or p.shape != self._shapes[k] or \
+                    p.device != self.device or rows_of(p) != self._rows[k] or p.is_neg():
                 raise ValueError(f"parameter {name!r} no longer has the type, shape, strides or device it was "
                                  "given with")
         both = overlapping(self._params, self._rows)
         if both is not None:
             raise ValueError(f"parameters {self.names[both[0]]!r} and {self.names[both[1]]!r} share memory")
-        self._aliases = [p.detach() for p in self._params]
-        self._ptrs = list(map(_data_ptr, self._params))
+        self._take_memory()
         self._entries["param"] = self._ptrs
 
     def _elements_in(self, entries: np.ndarray) -> bool:
@@ -399,7 +409,7 @@ class FusedAdamW:
                 found = [p.grad for p in params]
             else:
                 found = list(map(grads.get, names))
-            if list(map(_data_ptr, params)) != self._ptrs:
+            if not self._as_taken():
                 self._refresh()
             none = any(map(_is_none, found))
             if (none or (grads is not None and len(grads) != len(found))) and grads is not None and \

@@ -31,6 +31,12 @@ int dense_type(const at::Tensor& t, int device) {
     return type_code(t.scalar_type());
 }
 
+// Whether ``p`` still has the type, shape and strides of ``was``.
+bool same_form(const at::Tensor& p, const at::Tensor& was) {
+    return p.defined() && p.layout() == at::kStrided && p.scalar_type() == was.scalar_type() &&
+           p.sizes() == was.sizes() && p.strides() == was.strides() && !p.is_neg();
+}
+
 void changed(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -44,7 +50,8 @@ struct Span {
 
 // Fills ``e[k].grad`` and its type and row stride from the k-th of ``n`` tensors
 // shaped like ``like[k]``: those of the list ``items``, or those of the dict
-// ``items`` under ``names``, or (None) the ``grad`` of ``owners[k]``.
+// ``items`` under ``names``, or (None) the ``grad`` of ``owners[k]``.  ``owners``, where
+// given, must still have the form of ``like``.
 extern "C" int gst_fill(PyObject* items, PyObject* names, PyObject* owners, PyObject* like, gs_tensor* e, Py_ssize_t n,
                         int device) {
     try {
@@ -52,17 +59,20 @@ extern "C" int gst_fill(PyObject* items, PyObject* names, PyObject* owners, PyOb
         if (!(list || dict || items == Py_None) || !PyList_Check(like) || PyList_GET_SIZE(like) != n ||
             (list && PyList_GET_SIZE(items) != n) ||
             (dict && (PyDict_GET_SIZE(items) != n || !PyList_Check(names) || PyList_GET_SIZE(names) != n)) ||
-            (items == Py_None && (!PyList_Check(owners) || PyList_GET_SIZE(owners) != n)))
+            (items == Py_None && owners == Py_None) ||
+            (owners != Py_None && (!PyList_Check(owners) || PyList_GET_SIZE(owners) != n)))
             return 1;
         for (Py_ssize_t k = 0; k < n; ++k) {
             const at::Tensor* p = tensor_of(PyList_GET_ITEM(like, k));
             if (!p) return 1;
             const at::Tensor *g = nullptr, *owner = nullptr;
+            if (owners != Py_None && (!(owner = tensor_of(PyList_GET_ITEM(owners, k))) || !same_form(*owner, *p)))
+                return 1;
             if (list)
                 g = tensor_of(PyList_GET_ITEM(items, k));
             else if (dict)
                 g = tensor_of(PyDict_GetItem(items, PyList_GET_ITEM(names, k)));
-            else if ((owner = tensor_of(PyList_GET_ITEM(owners, k))))
+            else
                 g = &owner->grad();
             if (!g) return 1;
             const int type = dense_type(*g, device);

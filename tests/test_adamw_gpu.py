@@ -758,3 +758,38 @@ def test_gradients_that_autograd_negates(reader):
     ref = Reference(opt, params)
     opt.step(grads)
     ref.check(grads)
+
+
+# ---------------------------------------------------------------- parameters whose memory is laid out anew
+def test_parameters_laid_out_anew_at_their_address(reader):
+    """The address alone does not make a parameter the one that was given: another
+    layout or type there is refused, and the old form is taken again."""
+    params = {"a": torch.nn.Parameter(torch.randn(12, 12, device=DEV)),
+              "b": torch.nn.Parameter(torch.randn(30, device=DEV).to(F16))}
+    opt = FusedAdamW(params)
+    ref = Reference(opt, params)
+    grads = tensors(2, {"a": (12, 12), "b": (30,)}, F32)
+    first = {k: p.data for k, p in params.items()}
+    before = {k: p.detach().clone() for k, p in params.items()}
+    for name, other in (("a", first["a"].t()), ("b", first["b"].view(BF16)), ("a", first["a"][:, :4]),
+                        ("a", first["a"].view(144)), ("a", first["a"].view(18, 8)), ("b", torch._neg_view(first["b"]))):
+        params[name].data = other
+        for given in (grads, {name: grads[name]}):
+            with pytest.raises(ValueError, match="no longer"):
+                opt.step(given)
+        params[name].data = first[name]
+        assert all(torch.equal(params[k], before[k]) for k in params) and opt.t == 0
+    for p, g in zip(params.values(), grads.values()):
+        p.grad = g.to(p.dtype)
+    params["a"].data = first["a"].t()
+    with pytest.raises(ValueError, match="no longer"):
+        opt.step()
+    params["a"].data = first["a"]
+    opt.step()
+    ref.check({k: p.grad for k, p in params.items()})
+    # a transposition in place is one too
+    x = torch.randn(8, 8, device=DEV)
+    opt = FusedAdamW({"x": x})
+    x.t_()
+    with pytest.raises(ValueError, match="no longer"):
+        opt.step({"x": torch.ones(8, 8, device=DEV)})
