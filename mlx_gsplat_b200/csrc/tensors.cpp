@@ -94,7 +94,8 @@ extern "C" int gst_params_unmoved(PyObject* params, const gs_tensor* e, Py_ssize
         if (!PyList_Check(params) || PyList_GET_SIZE(params) != n) return 1;
         for (Py_ssize_t k = 0; k < n; ++k) {
             const at::Tensor* p = tensor_of(PyList_GET_ITEM(params, k));
-            if (!p || p->const_data_ptr() != e[k].param) return 1;
+            // (an address to write to: memory shared with a lazy copy becomes the parameter's own)
+            if (!p || p->mutable_data_ptr() != e[k].param) return 1;
         }
         for (Py_ssize_t k = 0; k < n; ++k) changed(*tensor_of(PyList_GET_ITEM(params, k)));
         return 0;

@@ -327,3 +327,20 @@ def test_negated_gradients_are_resolved(strided):
         clip_gradients([g], 1.0)
     with pytest.raises(ValueError, match="negative"):
         FusedAdamW({"a": g})
+
+
+def test_native_reader_writes_no_lazy_copy():
+    """A parameter whose memory a lazy copy still shares gets its own when a step is to write it, and is then reported
+    as moved."""
+    native = _lib.tensors()
+    if native is None:
+        pytest.skip("helper not built")
+    e, t = np.zeros(1, _ENTRY), torch.arange(3.0)
+    e["param"] = t.data_ptr()
+    copy = torch._lazy_clone(t)
+    assert native.gst_params_unmoved([t], e.ctypes.data, 1) == 1
+    assert t.data_ptr() != e["param"][0]
+    e["param"] = t.data_ptr()
+    assert native.gst_params_unmoved([t], e.ctypes.data, 1) == 0
+    t.zero_()
+    assert copy.tolist() == [0.0, 1.0, 2.0]

@@ -793,3 +793,19 @@ def test_parameters_laid_out_anew_at_their_address(reader):
     x.t_()
     with pytest.raises(ValueError, match="no longer"):
         opt.step({"x": torch.ones(8, 8, device=DEV)})
+
+
+def test_a_copy_made_lazily_is_not_stepped(reader):
+    """A parameter that shares its memory with a lazy copy of it gets memory of its own when it is written."""
+    p = torch.randn(300, device=DEV)
+    before = p.clone()
+    opt = FusedAdamW({"p": p}, lr=0.1)
+    ref = Reference(opt, {"p": p})
+    copy = torch._lazy_clone(p)
+    g = tensors(2, {"p": (300,)}, F32)
+    opt.step(g)
+    ref.check(g, lr=0.1)
+    assert torch.equal(copy, before) and not torch.equal(p, before)
+    opt.step(g)  # from its new memory
+    ref.check(g, lr=0.1)
+    assert torch.equal(copy, before)
