@@ -236,8 +236,12 @@ typedef struct gs_adamw_state {
     uint8_t *m_exp, *v_exp;
     float* master;         /* optional float32 copies of 16-bit parameters (a slab like m): the update is
                               applied to them and the parameters are their rounding */
-    int64_t* control;      /* 2 values on the device, zeroed at first: the steps taken, and a counter of the kernel */
+    int64_t* control;      /* values on the device, zeroed at first: the steps taken, the kernel's own and, with
+                              ``counted``, one for each tensor of a call: the steps that passed without its grad
+                              (set from outside: control[1] = 1 << 32 tells the kernel to look at them) */
     int32_t bits;
+    int32_t counted;       /* 0: every tensor counts every step.  1: each counts its own.  A call then names all tensors,
+                              always in the same order; one with a null grad is left as it is and misses the step */
 } gs_adamw_state;
 
 typedef struct gs_adamw_settings {
@@ -254,7 +258,8 @@ typedef struct gs_adamw_settings {
 } gs_adamw_settings;
 
 /* One AdamW step over all tensors: with c = grad_scale, times max_norm / norm
- * when clipped, and t the new step count,
+ * when clipped, and t the new step count (with ``counted``, less the steps that the
+ * tensor missed),
  *   g = c * grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
  *   param = (1 - lr decay) param - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
  * in float32: every operation of the moments rounded by itself, the square root

@@ -61,7 +61,7 @@ class GsRasterSettings(ctypes.Structure):
 
 class GsAdamWState(ctypes.Structure):
     _fields_ = [("m", c_vp), ("v", c_vp), ("m_exp", c_vp), ("v_exp", c_vp), ("master", c_vp), ("control", c_vp),
-                ("bits", i32)]
+                ("bits", i32), ("counted", i32)]
 
 
 class GsAdamWSettings(ctypes.Structure):

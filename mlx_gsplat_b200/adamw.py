@@ -183,6 +183,10 @@ class FusedAdamW:
     ``skip_nonfinite``: leave parameters, moments and the step count as they
     are when a gradient is not finite (a step with ``max_norm`` always does).
 
+    A parameter without a gradient in a step keeps its values and moments and
+    does not count the step: its bias corrections are those of the steps that
+    it took itself.
+
     Parameters may be strided rows (a pool's columns); they may not overlap.
     ``lr``, ``weight_decay``, ``beta1``, ``beta2``, ``eps``, ``max_norm`` and
     ``skip_nonfinite`` may be changed between steps (a captured step keeps the
@@ -255,15 +259,17 @@ class FusedAdamW:
         blocks = self.slab_elements // BLOCK if state_bits == 8 else 0
         self.m_exp = torch.zeros(blocks, dtype=torch.uint8, device=self.device)
         self.v_exp = torch.zeros(blocks, dtype=torch.uint8, device=self.device)
-        self._control = torch.zeros(2, dtype=torch.int64, device=self.device)
-        self._count = self._control[0]
+        # steps taken, the kernel's own (upper half: look at what follows), per parameter the steps without its gradient
+        self._control = torch.zeros(2 + n, dtype=torch.int64, device=self.device)
+        self._count, self._missed = self._control[0], self._control[2:]
+        self._any_missed = False  # whether any call so far left a parameter out
         self.master_slab: Optional[torch.Tensor] = None
         if master_weights and any(p.dtype != torch.float32 for p in self._params):
             self.master_slab = torch.zeros(self.slab_elements, dtype=torch.float32, device=self.device)
             self.sync_master()
         self._state = _lib.GsAdamWState(_lib.ptr(self.m), _lib.ptr(self.v), _lib.ptr(self.m_exp),
                                         _lib.ptr(self.v_exp), _lib.ptr(self.master_slab), _lib.ptr(self._control),
-                                        state_bits)
+                                        state_bits, 1)
         self._partials: Optional[torch.Tensor] = None
         if max_norm is not None or skip_nonfinite:
             self._partials_buffer(_lib.lib())
@@ -363,6 +369,8 @@ class FusedAdamW:
                     raise ValueError(f"{what} of {name!r} has shape {tuple(g.shape)}, not {tuple(s)}")
         if not here:
             raise ValueError(f"every {what} must be on {self.device}")
+        if ((entries["grad"] == 0) & (entries["n"] > 0)).any():
+            raise ValueError(f"a {what} has no memory")
         entries["grad_type"] = codes
         entries["grad_stride"] = entries["cols"]
         if not dense:
@@ -386,7 +394,7 @@ class FusedAdamW:
     def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_scale: float = 1.0) -> Optional[torch.Tensor]:
         """One step on the current stream.  ``grads``: name -> gradient (default:
         the parameters' ``.grad``); a parameter without one keeps its values and
-        moments, and a step without any does nothing.  ``grad_scale`` multiplies
+        moments and misses the step, and a step without any does nothing.  ``grad_scale`` multiplies
         every gradient first (the inverse of a loss scale).  Returns the global
         norm of the scaled gradients before clipping as a device scalar when
         ``max_norm`` or ``skip_nonfinite`` asks for it, else None."""
@@ -398,7 +406,7 @@ class FusedAdamW:
             raise ValueError(f"grad_scale must be finite: {grad_scale}")
         lr, lr_device = self._lr_value()
         limit = self._norm_limit()
-        names, shapes, params, entries = self.names, self._shapes, self._params, self._entries
+        names, shapes, params, entries, on = self.names, self._shapes, self._params, self._entries, None
         native = _lib.tensors()
         # every gradient there, dense and as expected: the table is filled natively
         filled = native is not None and \
@@ -428,15 +436,20 @@ class FusedAdamW:
                 return norm.zero_() if with_norm else None
             if not filled:
                 entries, keep = self._with_grads(entries, names, shapes, found)
-            at = self._at if entries is self._entries else entries.ctypes.data
+            at, count = self._at if entries is self._entries else entries.ctypes.data, len(entries)
             stream = _lib.stream_ptr(self.device)
             s = _lib.GsAdamWSettings(lr, self.beta1, self.beta2, self.eps, grad_scale, lr_device, None, 0, limit, None)
             if with_norm:
                 buffer = self._partials_buffer(lib)
-                s.num_partials = _norm_partials(lib, at, len(entries), buffer, stream)
+                s.num_partials = _norm_partials(lib, at, count, buffer, stream)
                 s.norm_partials = buffer.data_ptr()
                 s.norm_out = norm.data_ptr()
-            _lib.check(lib.gs_adamw_step(at, len(entries), self._state, s, stream), "adamw step")
+            if on is not None:  # the step takes the whole list, those that miss it without a gradient
+                every = self._entries.copy()
+                every["grad"] = 0
+                every[on] = entries
+                at, count, self._any_missed = every.ctypes.data, len(every), True
+            _lib.check(lib.gs_adamw_step(at, count, self._state, s, stream), "adamw step")
         if not filled:
             del keep
             _changed(params)
@@ -445,14 +458,20 @@ class FusedAdamW:
     # ------------------------------------------------------------------ state
     @property
     def t(self) -> int:
-        """Steps taken (read from the device: a host sync)."""
+        """Steps taken (read from the device: a host sync).  Setting it makes
+        every parameter one that took that many."""
         return int(self._count)
 
     @t.setter
     def t(self, value: int) -> None:
         if value < 0:
             raise ValueError(f"the step count must not be negative: {value}")
+        self._set_steps(value)
+
+    def _set_steps(self, value: int) -> None:
         self._count.fill_(int(value))
+        if self._any_missed:
+            self._control[1:].zero_()
 
     def _views(self, slab: torch.Tensor) -> Dict[str, torch.Tensor]:
         return {k: slab[self.offsets[k]:self.offsets[k] + s.numel()].view(s)
@@ -475,7 +494,7 @@ class FusedAdamW:
     def load_moments(self, m: Dict[str, torch.Tensor], v: Dict[str, torch.Tensor], t: Optional[int] = None) -> None:
         """Sets every parameter's moments (tensors of the parameters' shapes on
         their device, any of the three types; v must not be negative) and the
-        step count.  With 8-bit moments values that the form holds are kept
+        step count, which is then every parameter's (None: the counts stay).  With 8-bit moments values that the form holds are kept
         exactly and others are rounded with the step count's offsets."""
         if m.keys() != self.offsets.keys() or v.keys() != self.offsets.keys():
             raise ValueError("moments for exactly the optimizer's parameters are needed")
@@ -492,7 +511,7 @@ class FusedAdamW:
             if t is None:
                 t = self.t if self.state_bits == 8 else None
             else:
-                self._count.fill_(int(t))
+                self._set_steps(t)
             if self.state_bits == 32:
                 torch._foreach_copy_(list(self._views(self.m).values()) + list(self._views(self.v).values()), ml + vl)
                 return
@@ -515,8 +534,10 @@ class FusedAdamW:
 
     def state_dict(self) -> Dict[str, object]:
         """A copy of the state: the moments in the form they are held in, the
-        master copies, the step count and the layout."""
-        d = {"state_bits": self.state_bits, "t": self.t, "shapes": {k: tuple(s) for k, s in zip(self.names, self._shapes)},
+        master copies, the step count, the steps that each parameter missed and
+        the layout."""
+        d = {"state_bits": self.state_bits, "t": self.t, "missed": self._missed.clone(),
+             "shapes": {k: tuple(s) for k, s in zip(self.names, self._shapes)},
              "m": self.m.clone(), "v": self.v.clone(), "m_exp": self.m_exp.clone(), "v_exp": self.v_exp.clone()}
         if self.master_slab is not None:
             d["master"] = self.master_slab.clone()
@@ -539,10 +560,14 @@ class FusedAdamW:
             for dst, src in ((self.m, m), (self.v, v), (self.m_exp, d["m_exp"]), (self.v_exp, d["v_exp"])):
                 dst.copy_(src)
             self.t = d["t"]
-            return
-        if bits == 8:
-            m, v = _dequantize(m, v, d["m_exp"].to(self.device), d["v_exp"].to(self.device), torch.float32)
-        self.load_moments(self._views(m), self._views(v), t=d["t"])
+        else:
+            if bits == 8:
+                m, v = _dequantize(m, v, d["m_exp"].to(self.device), d["v_exp"].to(self.device), torch.float32)
+            self.load_moments(self._views(m), self._views(v), t=d["t"])
+        if "missed" in d:
+            self._missed.copy_(d["missed"])
+            self._control[1].fill_(1 << 32)
+            self._any_missed = True
 
 
 def _dequantize(m, v, m_exp, v_exp, dtype) -> Tuple[torch.Tensor, torch.Tensor]:

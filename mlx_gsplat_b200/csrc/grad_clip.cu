@@ -147,21 +147,19 @@ __global__ void __launch_bounds__(kMultiThreads) grad_clip_kernel(const __grid_c
 }
 
 template <int kCap>
-static int norm_launches(const gs_tensor* t, int64_t count, double* partials, int64_t capacity, int64_t* written,
-                         bool launch, cudaStream_t stream) {
+static int norm_launches(const gs_tensor* t, int64_t count, int64_t left, double* partials, int64_t capacity,
+                         int64_t* written, cudaStream_t stream) {
     TensorTable<kCap> tab;
-    int64_t left = live_tensors(t, count), done = 0;
+    int64_t done = 0;
     for (int64_t at = 0; left > 0;) {
         at = fill_table(tab, t, at, count);
         left -= tab.count;
         const int grid = table_grid(tab, kNormBlocksPerSm, kNormGroup);
-        if (launch) {
-            if (done + grid > capacity)
-                return set_error(GS_ERR_CAPACITY, "grad_norm: %lld partial sums do not fit", (long long)capacity);
-            double* out = partials + done;
-            void* args[] = {&tab, &out};
-            GS_TRY(launch_table("grad_norm_kernel", (const void*)grad_norm_kernel<kCap>, grid, stream, args));
-        }
+        if (done + grid > capacity)
+            return set_error(GS_ERR_CAPACITY, "grad_norm: %lld partial sums do not fit", (long long)capacity);
+        double* out = partials + done;
+        void* args[] = {&tab, &out};
+        GS_TRY(launch_table("grad_norm_kernel", (const void*)grad_norm_kernel<kCap>, grid, stream, args));
         done += grid;
     }
     *written = done;
@@ -169,10 +167,9 @@ static int norm_launches(const gs_tensor* t, int64_t count, double* partials, in
 }
 
 template <int kCap>
-static int clip_launches(const gs_tensor* t, int64_t count, const double* partials, int64_t num_partials,
-                         double max_norm, float* norm_out, cudaStream_t stream) {
+static int clip_launches(const gs_tensor* t, int64_t count, int64_t left, const double* partials,
+                         int64_t num_partials, double max_norm, float* norm_out, cudaStream_t stream) {
     TensorTable<kCap> tab;
-    int64_t left = live_tensors(t, count);
     for (int64_t at = 0; left > 0;) {
         at = fill_table(tab, t, at, count);
         left -= tab.count;
@@ -198,24 +195,26 @@ extern "C" int gs_grad_norm_partials(const gs_tensor* tensors, int64_t count, do
                                      int64_t* num_partials, gs_stream_t stream) {
     GS_REQUIRE(num_partials, "grad_norm: null count");
     *num_partials = 0;
-    GS_TRY(check_tensors("grad_norm", tensors, count, kNeedGrad));
-    if (live_tensors(tensors, count) == 0) return GS_OK;
+    int64_t live;
+    GS_TRY(check_tensors("grad_norm", tensors, count, kNeedGrad, live));
+    if (live == 0) return GS_OK;
     GS_REQUIRE(partials && capacity > 0, "grad_norm: null partial sums");
     const cudaStream_t st = (cudaStream_t)stream;
     return count <= kSmallTable
-               ? norm_launches<kSmallTable>(tensors, count, partials, capacity, num_partials, true, st)
-               : norm_launches<kLargeTable>(tensors, count, partials, capacity, num_partials, true, st);
+               ? norm_launches<kSmallTable>(tensors, count, live, partials, capacity, num_partials, st)
+               : norm_launches<kLargeTable>(tensors, count, live, partials, capacity, num_partials, st);
 }
 
 extern "C" int gs_clip_gradients(const gs_tensor* tensors, int64_t count, const double* partials,
                                  int64_t num_partials, double max_norm, float* norm_out, gs_stream_t stream) {
     GS_REQUIRE(max_norm > 0.0, "clip_gradients: max_norm must be positive");
     GS_REQUIRE(num_partials >= 0, "clip_gradients: bad partial count");
-    GS_TRY(check_tensors("clip_gradients", tensors, count, kNeedParam | kNeedGrad));
-    if (live_tensors(tensors, count) == 0) return GS_OK;
+    int64_t live;
+    GS_TRY(check_tensors("clip_gradients", tensors, count, kNeedParam | kNeedGrad, live));
+    if (live == 0) return GS_OK;
     GS_REQUIRE(partials, "clip_gradients: null partial sums");
     const cudaStream_t st = (cudaStream_t)stream;
     return count <= kSmallTable
-               ? clip_launches<kSmallTable>(tensors, count, partials, num_partials, max_norm, norm_out, st)
-               : clip_launches<kLargeTable>(tensors, count, partials, num_partials, max_norm, norm_out, st);
+               ? clip_launches<kSmallTable>(tensors, count, live, partials, num_partials, max_norm, norm_out, st)
+               : clip_launches<kLargeTable>(tensors, count, live, partials, num_partials, max_norm, norm_out, st);
 }

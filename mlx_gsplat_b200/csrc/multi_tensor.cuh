@@ -30,6 +30,7 @@ struct TensorEntry {
     double lr_scale, decay;
     int16_t param_type, grad_type;
     int8_t param_vec, grad_vec;  // dense and aligned for accesses to eight elements
+    uint16_t place;              // in the caller's list, counted from the table's first tensor
 };
 
 // Table sizes: a small one for the handful of tensors of a scene (a 2 KB
@@ -379,14 +380,35 @@ inline bool can_vector(const void* p, int64_t n, int64_t cols, int64_t stride) {
     return (cols >= n || stride == cols) && aligned16(p);
 }
 
-enum { kNeedParam = 1, kNeedGrad = 2 };
+// What a call needs of its tensors; kMayMiss: those with a null grad are passed over.
+enum { kNeedParam = 1, kNeedGrad = 2, kMayMiss = 4 };
 
-// Checks the caller's entries (before anything is launched).
-inline int check_tensors(const char* what, const gs_tensor* t, int64_t count, int need) {
+inline bool passed_over(const gs_tensor& t) { return t.n == 0 || !t.grad; }
+
+inline bool sound_side(const void* p, int type, int64_t stride, int64_t cols) {
+    return (p != nullptr) & ((unsigned)type <= GS_F16) &
+           ((reinterpret_cast<uintptr_t>(p) & (type == GS_F32 ? 3u : 1u)) == 0) & (stride >= cols);
+}
+
+// Whether an entry takes part and is without a fault (one expression: a call over a few
+// hundred short tensors spends more here than the device does).
+inline bool sound_entry(const gs_tensor& e, int need) {
+    return ((uint64_t)e.n - 1 < (uint64_t)1 << 40) & (e.cols > 0) & (e.state >= 0) & (e.state % GS_MOMENT_BLOCK == 0) &
+           (!(need & kNeedParam) || sound_side(e.param, e.param_type, e.param_stride, e.cols)) &
+           sound_side(e.grad, e.grad_type, e.grad_stride, e.cols);
+}
+
+// Checks the caller's entries (before anything is launched) and counts those that take part.
+inline int check_tensors(const char* what, const gs_tensor* t, int64_t count, int need, int64_t& live) {
+    live = 0;
     GS_REQUIRE(count >= 0, "%s: negative tensor count", what);
     GS_REQUIRE(count == 0 || t, "%s: null tensor list", what);
     for (int64_t k = 0; k < count; ++k) {
         const gs_tensor& e = t[k];
+        if (sound_entry(e, need)) {
+            ++live;
+            continue;
+        }
         GS_REQUIRE(e.n >= 0 && e.n <= ((int64_t)1 << 40), "%s: tensor %lld: bad element count %lld", what, (long long)k,
                    (long long)e.n);
         if (e.n == 0) continue;
@@ -399,6 +421,7 @@ inline int check_tensors(const char* what, const gs_tensor* t, int64_t count, in
             const int type = q ? e.grad_type : e.param_type;
             const int64_t stride = q ? e.grad_stride : e.param_stride;
             const char* name = q ? "grad" : "param";
+            if (q && !p && (need & kMayMiss)) continue;
             GS_REQUIRE(p, "%s: tensor %lld: null %s", what, (long long)k, name);
             GS_REQUIRE(type == GS_F32 || type == GS_BF16 || type == GS_F16, "%s: tensor %lld: unknown %s type %d", what,
                        (long long)k, name, type);
@@ -411,15 +434,19 @@ inline int check_tensors(const char* what, const gs_tensor* t, int64_t count, in
     return GS_OK;
 }
 
-// Fills a table with up to kCap non-empty tensors from t[at]; returns the next place.
+// Fills a table with up to kCap tensors that have elements and a grad from t[at]; returns
+// the next place.
 template <int kCap>
 inline int64_t fill_table(TensorTable<kCap>& tab, const gs_tensor* t, int64_t at, int64_t count) {
     int k = 0;
     int64_t chunks = 0;
+    int64_t from = at;
     tab.all_vec = 1;
     for (; at < count && k < kCap; ++at) {
         const gs_tensor& s = t[at];
-        if (s.n == 0) continue;
+        if (passed_over(s)) continue;
+        if (k == 0) from = at;
+        if (at - from > 0xffff) break;
         const int64_t c = (s.n + kChunk - 1) / kChunk;
         if (chunks + c > 0x7f000000) break;
         TensorEntry& e = tab.e[k];
@@ -432,6 +459,7 @@ inline int64_t fill_table(TensorTable<kCap>& tab, const gs_tensor* t, int64_t at
         e.grad_stride = s.grad_stride;
         e.lr_scale = s.lr_scale;
         e.decay = s.decay;
+        e.place = (uint16_t)(at - from);
         e.param_type = (int16_t)s.param_type;
         e.grad_type = (int16_t)s.grad_type;
         e.param_vec = can_vector(s.param, s.n, s.cols, s.param_stride);
@@ -444,12 +472,6 @@ inline int64_t fill_table(TensorTable<kCap>& tab, const gs_tensor* t, int64_t at
     tab.first[k] = (int32_t)chunks;
     tab.count = k;
     return at;
-}
-
-inline int64_t live_tensors(const gs_tensor* t, int64_t count) {
-    int64_t k = 0;
-    for (int64_t i = 0; i < count; ++i) k += t[i].n > 0;
-    return k;
 }
 
 // Blocks for a table and the size of their groups: at most one wave of resident

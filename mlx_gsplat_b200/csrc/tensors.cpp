@@ -31,10 +31,17 @@ int dense_type(const at::Tensor& t, int device) {
     return type_code(t.scalar_type());
 }
 
-// Whether ``p`` still has the type, shape and strides of ``was``.
+// Whether ``p`` still has the type, shape and strides of ``was``, a strided tensor (the
+// sizes of other layouts throw).
 bool same_form(const at::Tensor& p, const at::Tensor& was) {
-    return p.defined() && p.layout() == at::kStrided && p.scalar_type() == was.scalar_type() &&
-           p.sizes() == was.sizes() && p.strides() == was.strides() && !p.is_neg();
+    const auto *a = p.unsafeGetTensorImpl(), *b = was.unsafeGetTensorImpl();
+    const int64_t n = a->dim();
+    if (n != b->dim() || a->dtype() != b->dtype() || p.is_neg()) return false;
+    const int64_t *size = a->sizes().data(), *stride = a->strides().data();
+    const int64_t *size0 = b->sizes().data(), *stride0 = b->strides().data();
+    for (int64_t k = 0; k < n; ++k)
+        if ((size[k] != size0[k]) | (stride[k] != stride0[k])) return false;
+    return true;
 }
 
 void changed(const at::Tensor& t) {
@@ -78,6 +85,7 @@ extern "C" int gst_fill(PyObject* items, PyObject* names, PyObject* owners, PyOb
             const int type = dense_type(*g, device);
             if (type < 0 || g->sizes() != p->sizes()) return 1;
             e[k].grad = g->const_data_ptr();
+            if (!e[k].grad && g->numel() > 0) return 1;
             e[k].grad_type = type;
             e[k].grad_stride = e[k].cols;
         }
@@ -97,7 +105,7 @@ extern "C" int gst_params_unmoved(PyObject* params, const gs_tensor* e, Py_ssize
             // (an address to write to: memory shared with a lazy copy becomes the parameter's own)
             if (!p || p->mutable_data_ptr() != e[k].param) return 1;
         }
-        for (Py_ssize_t k = 0; k < n; ++k) changed(*tensor_of(PyList_GET_ITEM(params, k)));
+        for (Py_ssize_t k = 0; k < n; ++k) changed(THPVariable_Unpack(PyList_GET_ITEM(params, k)));
         return 0;
     } catch (...) {
         return 1;

@@ -344,3 +344,16 @@ def test_native_reader_writes_no_lazy_copy():
     assert native.gst_params_unmoved([t], e.ctypes.data, 1) == 0
     t.zero_()
     assert copy.tolist() == [0.0, 1.0, 2.0]
+
+
+@built
+def test_counted_calls_pass_over_null_gradients():
+    lib = _lib.load()
+    e, state = _entry(grad=0), _state()
+    assert lib.gs_adamw_step(e.ctypes.data, 1, state, _settings(), None) == _lib.GS_ERR_INVALID
+    state.counted = 1
+    assert lib.gs_adamw_step(e.ctypes.data, 1, state, _settings(), None) == 0  # no gradient: nothing to do
+    state.counted = 2
+    assert lib.gs_adamw_step(e.ctypes.data, 1, state, _settings(), None) == _lib.GS_ERR_INVALID
+    assert b"counted" in lib.gs_last_error()
+    assert lib.gs_grad_norm_partials(e.ctypes.data, 1, 4096, 8, ctypes.byref(ctypes.c_int64()), None) == _lib.GS_ERR_INVALID

@@ -809,3 +809,168 @@ def test_a_copy_made_lazily_is_not_stepped(reader):
     opt.step(g)  # from its new memory
     ref.check(g, lr=0.1)
     assert torch.equal(copy, before)
+
+
+# ---------------------------------------------------------------- parameters that miss steps
+class CountedReference:
+    """The definition with a step count for every tensor: a tensor without a
+    gradient keeps its values and moments and does not count the step."""
+
+    def __init__(self, opt, params):
+        self.opt, self.params = opt, params
+        self.p = {k: flat(p) for k, p in params.items()}
+        self.m, self.v = ({k: np.zeros(p.size, np.float32) for k, p in self.p.items()} for _ in range(2))
+        self.count = dict.fromkeys(params, 0)
+        self.t = 0
+
+    def check(self, grads, lr, scale=1.0):
+        o = self.opt
+        self.t += any(g.numel() for g in grads.values())  # without an element to move a step does nothing
+        got_m, got_v = o.moments()
+        for k in self.params:
+            if k in grads:
+                self.count[k] += 1
+                gg = flat(grads[k])
+                args = dict(beta1=o.beta1, beta2=o.beta2, scale=scale)
+                pn, _, _, bound = oadamw.step64(self.p[k], gg, self.m[k], self.v[k], lr=lr, eps=o.eps,
+                                                decay=o.weight_decay, t=self.count[k], **args)
+                self.m[k], self.v[k] = oadamw.step32(gg, self.m[k], self.v[k], **args)
+                if o.state_bits == 8:  # the roundings' offsets are those of the optimizer's steps
+                    self.m[k] = oadamw.values(*oadamw.quantize(self.m[k], self.t, False), False)[:gg.size]
+                    self.v[k] = oadamw.values(*oadamw.quantize(self.v[k], self.t, True), True)[:gg.size]
+                got = flat(self.params[k])
+                err = np.abs(got - pn)
+                assert (err <= bound).all(), (k, self.t, (err / np.maximum(bound, 1e-300)).max())
+                self.p[k] = got
+            else:
+                np.testing.assert_array_equal(flat(self.params[k]), self.p[k], err_msg=k)
+            np.testing.assert_array_equal(flat(got_m[k]), self.m[k], err_msg=f"m of {k}")
+            np.testing.assert_array_equal(flat(got_v[k]), self.v[k], err_msg=f"v of {k}")
+        assert o.t == self.t
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("count", [4, 40, 400])
+def test_missed_steps_are_not_counted(bits, count, reader):
+    """Late and rare gradients get the bias corrections of the steps that their
+    own tensor took; one tensor spans many blocks, and tables and lists of
+    missing tensors are passed."""
+    rng = np.random.default_rng(count)
+    shapes = {f"x{i}": (int(n),) for i, n in enumerate(rng.integers(1, 700, count))}
+    shapes["x1"], shapes["x2"] = (1_300_001,), (0,)
+    params = tensors(1, shapes, F32)
+    opt = FusedAdamW(params, lr=1e-2, state_bits=bits)
+    ref = CountedReference(opt, params)
+    for s in range(5):
+        grads = tensors(10 + s, shapes, F32, scale=1e-2)
+        if s != 3:  # the fourth step has all of them
+            grads = {k: g for i, (k, g) in enumerate(grads.items()) if (i + s) % 3 == 0 or (i == 1 and s == 4)}
+        opt.step(grads)
+        ref.check(grads, lr=1e-2)
+
+
+def test_missed_steps_of_very_many_tensors():
+    """More tensors in a list than a table's 16-bit places span."""
+    n = 70_001
+    gen = torch.Generator().manual_seed(0)
+    p, g, g2 = (torch.randn(n, generator=gen).to(DEV) for _ in range(3))
+    zero = np.zeros(n)
+    params = {f"x{i}": x for i, x in enumerate(p.split(1))}
+    opt = FusedAdamW(params, lr=0.1)
+    ends = [0, n - 1]
+    p0 = flat(p)
+    opt.step({f"x{i}": g[i:i + 1] for i in ends})
+    args = dict(lr=0.1, beta1=0.9, beta2=0.999, eps=1e-8, decay=0.01)
+    p1, m1, v1, bound = oadamw.step64(p0, flat(g), zero, zero, t=1, **args)
+    got = flat(p)
+    assert (np.abs(got - p1) <= bound)[ends].all() and (got == p0)[1:-1].all()
+    opt.step({f"x{i}": x for i, x in enumerate(g2.split(1))})
+    m, v = (np.zeros(n, np.float32) for _ in range(2))
+    mm, vv = oadamw.step32(flat(g), m, v, beta1=0.9, beta2=0.999)
+    m[ends], v[ends] = mm[ends], vv[ends]
+    late, _, _, bound_late = oadamw.step64(got, flat(g2), m, v, t=1, **args)
+    early, _, _, bound_early = oadamw.step64(got, flat(g2), m, v, t=2, **args)
+    assert (np.abs(flat(p) - early) <= bound_early)[ends].all()
+    assert (np.abs(flat(p) - late) <= bound_late)[1:-1].all()
+
+
+@pytest.mark.parametrize("kw", [dict(max_norm=0.5), dict(skip_nonfinite=True)])
+def test_skipped_steps_are_missed_by_nobody(kw):
+    shapes = {"a": (700,), "b": (3000,)}
+    params = tensors(1, shapes, F32)
+    opt = FusedAdamW(params, lr=1e-2, **kw)
+    ref = CountedReference(opt, params)
+    for s in range(4):
+        grads = tensors(10 + s, shapes, F32)
+        if s < 2:
+            del grads["b"]
+        exact = math.sqrt(sum(float(g.double().square().sum()) for g in grads.values()))
+        bad = {k: g.clone() for k, g in grads.items()}
+        bad["a"][3] = math.nan
+        opt.step(bad)
+        opt.step(grads)
+        ref.check(grads, lr=1e-2, scale=min(1.0, 0.5 / exact) if "max_norm" in kw else 1.0)
+
+
+def test_missed_steps_in_a_graph_and_in_the_state():
+    shapes = {"a": (700,), "b": (3000,), "c": (5,)}
+    params = tensors(1, shapes, F32)
+    opt = FusedAdamW(params, lr=1e-2)
+    ref = CountedReference(opt, params)
+    static = {k: g.clone() for k, g in tensors(5, shapes, F32).items()}
+    opt.step(static)
+    ref.check(static, lr=1e-2)
+    # one graph with every gradient, captured before any was missed, and one without b's
+    every, some = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(every):
+        opt.step(static)
+    part = {k: static[k] for k in "ac"}
+    with torch.cuda.graph(some):
+        opt.step(part)
+    for s, graph in enumerate([every, some, some, every, some, every]):
+        for k, g in tensors(20 + s, shapes, F32).items():
+            static[k].copy_(g)
+        graph.replay()
+        ref.check(part if graph is some else static, lr=1e-2)
+    # resumed, in either form's number of bits
+    d = opt.state_dict()
+    for bits in (32, 8):
+        again = FusedAdamW({k: p.clone() for k, p in params.items()}, lr=1e-2, state_bits=bits)
+        again.load_state_dict(d)
+        more = CountedReference(again, dict(zip(shapes, again._params)))
+        more.t, more.count = ref.t, dict(ref.count)
+        more.m, more.v = ({k: flat(x) for k, x in z.items()} for z in again.moments())
+        for part in ({"b": static["b"]}, static):
+            again.step(part)
+            more.check(part, lr=1e-2)
+    # a state without the counts, a set count and loaded moments: every tensor took those steps
+    old = {k: x for k, x in d.items() if k != "missed"}
+    for change in (lambda: again.load_state_dict(old), lambda: setattr(again, "t", 9),
+                   lambda: again.load_moments(*again.moments(), t=12)):
+        again.step({"a": static["a"]})
+        change()
+        more = CountedReference(again, dict(zip(shapes, again._params)))
+        more.t = again.t
+        more.count = dict.fromkeys(shapes, more.t)
+        more.m, more.v = ({k: flat(x) for k, x in z.items()} for z in again.moments())
+        again.step(static)
+        more.check(static, lr=1e-2)
+    # moments loaded without a count leave the counts
+    again.step({"a": static["a"]})
+    again.load_moments(*again.moments())
+    more = CountedReference(again, dict(zip(shapes, again._params)))
+    more.t = again.t
+    more.count = {"a": more.t, "b": more.t - 1, "c": more.t - 1}
+    more.m, more.v = ({k: flat(x) for k, x in z.items()} for z in again.moments())
+    again.step(static)
+    more.check(static, lr=1e-2)
+
+
+def test_a_gradient_without_memory_is_not_a_missing_one(reader):
+    params = {"a": torch.zeros(8, device=DEV), "b": torch.zeros(8, device=DEV)}
+    opt = FusedAdamW(params)
+    none = torch._efficientzerotensor((8,), device=DEV)
+    for grads in ({"a": none, "b": torch.ones(8, device=DEV)}, {"a": none}):
+        with pytest.raises(ValueError, match="no memory"):
+            opt.step(grads)
+    assert opt.t == 0
