@@ -7,6 +7,8 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
+import warnings
 from typing import Optional
 
 import torch
@@ -174,20 +176,48 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 
 _TENSORS: Optional[ctypes.PyDLL] = None
+_TENSORS_DECIDED = False
+
+
+def tensors_abi() -> str:
+    """What the tensor helper is compiled against: it reads the insides of
+    torch's tensors, which change between versions."""
+    return f"torch {torch.__version__}, python {sys.version_info.major}.{sys.version_info.minor}"
+
+
+def load_tensors(path: str) -> ctypes.PyDLL:
+    """The helper at ``path``; OSError where it cannot be loaded or was compiled
+    against another torch or Python."""
+    dll = ctypes.PyDLL(path)
+    try:
+        dll.gst_abi.restype = ctypes.c_char_p
+        abi = dll.gst_abi().decode()
+    except AttributeError:
+        abi = "an unknown torch"
+    if not all(hasattr(dll, name) for name in ("gst_fill", "gst_params_unmoved", "gst_clip")):
+        raise OSError(f"{path} is not the tensor helper")
+    if abi != tensors_abi():
+        raise OSError(f"{path} was compiled against {abi}, not {tensors_abi()}")
+    obj, size = ctypes.py_object, ctypes.c_ssize_t
+    dll.gst_fill.argtypes = [obj, obj, obj, obj, c_vp, size, ctypes.c_int]
+    dll.gst_params_unmoved.argtypes = [obj, c_vp, size]
+    dll.gst_clip.argtypes = [obj, obj, c_vp, size, ctypes.POINTER(ctypes.c_int)]
+    return dll
 
 
 def tensors() -> Optional[ctypes.PyDLL]:
     """The helper that reads tensors' metadata natively (``csrc/tensors.cpp``;
-    called with the GIL held), or None where it was not built: the callers' own
-    checks in Python then do the same."""
-    global _TENSORS
-    if _TENSORS is None and os.path.exists(TENSORS_PATH):
-        dll = ctypes.PyDLL(TENSORS_PATH)
-        obj, size = ctypes.py_object, ctypes.c_ssize_t
-        dll.gst_fill.argtypes = [obj, obj, obj, obj, c_vp, size, ctypes.c_int]
-        dll.gst_params_unmoved.argtypes = [obj, c_vp, size]
-        dll.gst_clip.argtypes = [obj, obj, c_vp, size, ctypes.POINTER(ctypes.c_int)]
-        _TENSORS = dll
+    called with the GIL held), or None where there is none for this torch: the
+    callers' own checks in Python then do the same.  Decided at the first call."""
+    global _TENSORS, _TENSORS_DECIDED
+    if not _TENSORS_DECIDED:
+        _TENSORS_DECIDED = True
+        if os.path.exists(TENSORS_PATH):
+            try:
+                _TENSORS = load_tensors(TENSORS_PATH)
+            except OSError as e:
+                warnings.warn(f"tensors are read in Python, not natively: {e}; rebuild with "
+                              "`python -m mlx_gsplat_b200.build`", RuntimeWarning, stacklevel=2)
     return _TENSORS
 
 

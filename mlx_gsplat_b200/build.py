@@ -4,7 +4,8 @@ Usage: ``python -m mlx_gsplat_b200.build`` (or ``build()`` from Python).
 The library is a plain C ABI (``include/gsplat_b200.h``) loaded with ctypes;
 no PyTorch headers are involved.  Beside it ``libgsplat_tensors.so``
 (``csrc/tensors.cpp``, g++ with torch's headers) reads torch tensors' metadata
-for the many-tensor calls; it holds no kernels.
+for the many-tensor calls; it holds no kernels, and where it cannot be compiled
+the package does the same in Python.
 """
 from __future__ import annotations
 
@@ -47,11 +48,14 @@ def build_tensors() -> str:
     import sysconfig
 
     import torch
+
+    from . import _lib
     root = os.path.dirname(torch.__file__)
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                 sysconfig.get_paths()["include"]]
     tmp = TENSORS_LIB + ".tmp"
     cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f'-DGST_ABI="{_lib.tensors_abi()}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in includes),
            "-I", INCLUDE, TENSORS_SRC, "-o", tmp, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
            "-lc10"]
@@ -62,19 +66,48 @@ def build_tensors() -> str:
     return TENSORS_LIB
 
 
+def _older(lib, deps) -> bool:
+    return not os.path.exists(lib) or any(os.path.getmtime(d) > os.path.getmtime(lib) for d in deps)
+
+
+def _headers():
+    return glob.glob(os.path.join(INCLUDE, "*.h"))
+
+
 def _stale(objs, srcs) -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(TENSORS_LIB):
+    return _older(LIB, srcs + glob.glob(os.path.join(CSRC, "*.cuh")) + _headers())
+
+
+def _tensors_stale() -> bool:
+    if _older(TENSORS_LIB, [TENSORS_SRC] + _headers()):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(TENSORS_LIB))
-    deps = srcs + [TENSORS_SRC] + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
-    return any(os.path.getmtime(d) > t for d in deps)
+    from . import _lib
+    try:
+        _lib.load_tensors(TENSORS_LIB)
+    except OSError:  # compiled against another torch
+        return True
+    return False
+
+
+def _try_tensors() -> None:
+    """Compiles the tensor helper; without it (no g++, no headers of torch or
+    Python) the rest of the package works the same."""
+    try:
+        build_tensors()
+    except (RuntimeError, OSError) as e:
+        if os.path.exists(TENSORS_LIB):
+            os.remove(TENSORS_LIB)  # of other sources or another torch
+        print(f"the tensor helper was not built, tensors will be read in Python: {e}", file=sys.stderr)
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     srcs = sources()
     os.makedirs(BUILD_DIR, exist_ok=True)
     objs = [os.path.join(BUILD_DIR, os.path.basename(s)[:-3] + ".o") for s in srcs]
+    helper = force or _tensors_stale()
     if not force and not _stale(objs, srcs):
+        if helper:
+            _try_tensors()
         return LIB
     nvcc = _nvcc()
     flags = NVCC_FLAGS + list(extra_flags or [])
@@ -88,9 +121,10 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
         return r.stderr
 
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        tensors = ex.submit(build_tensors)
+        tensors = ex.submit(_try_tensors) if helper else None
         logs = list(ex.map(compile_one, zip(srcs, objs)))
-        tensors.result()
+        if tensors:
+            tensors.result()
     if verbose:
         for s, log in zip(srcs, logs):
             if log.strip():

@@ -55,6 +55,9 @@ struct Span {
 
 }  // namespace
 
+// What this file was compiled against: a loader refuses it under anything else.
+extern "C" const char* gst_abi() { return GST_ABI; }
+
 // Fills ``e[k].grad`` and its type and row stride from the k-th of ``n`` tensors
 // shaped like ``like[k]``: those of the list ``items``, or those of the dict
 // ``items`` under ``names``, or (None) the ``grad`` of ``owners[k]``.  ``owners``, where

@@ -3,6 +3,9 @@ the C ABI's argument checks, and the 8-bit form's properties (in the oracle)."""
 import ctypes
 import math
 import os
+import shutil
+import subprocess
+import warnings
 
 import numpy as np
 import pytest
@@ -357,3 +360,74 @@ def test_counted_calls_pass_over_null_gradients():
     assert lib.gs_adamw_step(e.ctypes.data, 1, state, _settings(), None) == _lib.GS_ERR_INVALID
     assert b"counted" in lib.gs_last_error()
     assert lib.gs_grad_norm_partials(e.ctypes.data, 1, 4096, 8, ctypes.byref(ctypes.c_int64()), None) == _lib.GS_ERR_INVALID
+
+
+# ---------------------------------------------------------------- the native reader's library
+@pytest.fixture
+def undecided(monkeypatch):
+    monkeypatch.setattr(_lib, "_TENSORS", None)
+    monkeypatch.setattr(_lib, "_TENSORS_DECIDED", False)
+
+
+def stub_helper(path, abi):
+    """A library at ``path`` that says it was compiled against ``abi`` (None: says nothing)."""
+    cc = shutil.which("cc") or shutil.which("gcc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    body = "int gst_fill(void) { return 7; }\n"
+    if abi is not None:
+        body += f'const char* gst_abi(void) {{ return "{abi}"; }}\n'
+    subprocess.run([cc, "-shared", "-fPIC", "-x", "c", "-", "-o", str(path)], input=body.encode(), check=True)
+
+
+@pytest.mark.parametrize("kind", ["another torch", "no version", "no library", "missing"])
+def test_unfit_helper_is_left_out(tmp_path, monkeypatch, undecided, kind):
+    """A helper of another torch, or one that does not load, is not called: tensors
+    are read in Python, and the reason is given once."""
+    path = tmp_path / "libgsplat_tensors.so"
+    if kind == "another torch":
+        stub_helper(path, "torch 1.0, python 3.0")
+    elif kind == "no version":
+        stub_helper(path, None)
+    elif kind == "no library":
+        path.write_text("not a library")
+    monkeypatch.setattr(_lib, "TENSORS_PATH", str(path))
+    with warnings.catch_warnings(record=True) as caught:
+        warnings.simplefilter("always")
+        assert _lib.tensors() is None and _lib.tensors() is None
+    assert len(caught) == (kind != "missing")
+    with pytest.raises(ValueError, match="CUDA"):  # and calls run without it
+        clip_gradients([torch.zeros(3)], 1.0)
+
+
+def test_helper_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
+    from mlx_gsplat_b200 import build
+    path = tmp_path / "libgsplat_tensors.so"
+    monkeypatch.setattr(build, "TENSORS_LIB", str(path))
+    assert build._tensors_stale()
+    stub_helper(path, _lib.tensors_abi())
+    os.utime(path, (2 ** 33, 2 ** 33))
+    assert build._tensors_stale()  # lacks the functions: not a helper that loads
+    stub = tmp_path / "other.so"
+    stub_helper(stub, "torch 1.0, python 3.0")
+    os.utime(stub, (2 ** 33, 2 ** 33))
+    monkeypatch.setattr(build, "TENSORS_LIB", str(stub))
+    assert build._tensors_stale()
+    if _lib.tensors() is not None:
+        monkeypatch.setattr(build, "TENSORS_LIB", _lib.TENSORS_PATH)
+        monkeypatch.setattr(build, "_older", lambda *a: False)
+        assert not build._tensors_stale()
+
+
+def test_build_does_without_the_helper(tmp_path, monkeypatch, capsys):
+    """Where the helper cannot be compiled the build goes on, and an old one is removed."""
+    from mlx_gsplat_b200 import build
+    path = tmp_path / "libgsplat_tensors.so"
+    path.write_text("of other sources")
+    monkeypatch.setattr(build, "TENSORS_LIB", str(path))
+    monkeypatch.setattr(build, "_stale", lambda *a: False)
+    monkeypatch.setenv("CXX", "/bin/false")
+    assert build.build() == build.LIB
+    assert not path.exists() and "read in Python" in capsys.readouterr().err
+    monkeypatch.setenv("CXX", str(tmp_path / "no such compiler"))
+    assert build.build() == build.LIB
