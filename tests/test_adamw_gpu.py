@@ -974,3 +974,113 @@ def test_a_gradient_without_memory_is_not_a_missing_one(reader):
         with pytest.raises(ValueError, match="no memory"):
             opt.step(grads)
     assert opt.t == 0
+
+
+# ---------------------------------------------------------------- rows and odd addresses in every type
+def laid_out(seed, count, dtype, scale=1.0):
+    """name -> tensor: columns of a slab, rows at a distance, odd and even offsets, dense and empty tensors; and the
+    buffers that they lie in, with a mask of what the tensors cover."""
+    gen = torch.Generator().manual_seed(seed)
+
+    def noise(*shape):
+        x = torch.randn(shape, generator=gen) * torch.exp(2 * torch.randn(shape, generator=gen)) * scale
+        return x.to(dtype).to(DEV)
+
+    out, backs, masks = {}, [], []
+
+    def add(back, *cuts):
+        mask = torch.zeros(back.shape, dtype=torch.bool, device=DEV)
+        for cut in cuts:
+            out[f"x{len(out)}"] = cut(back)
+            cut(mask).fill_(True)
+        backs.append(back)
+        masks.append(mask)
+
+    add(noise(303, 21), lambda b: b[:, 0:4], lambda b: b[:, 4:5], lambda b: b[1::3, 6:19])
+    add(noise(2600), lambda b: b[1:2566], lambda b: b[2570:2570])
+    add(noise(70, 97), lambda b: b[:, 3:92])  # rows longer than a warp's step
+    add(noise(4100), lambda b: b[:2049])
+    while len(out) < count:
+        n = int(torch.randint(1, 90, (), generator=gen))
+        add(noise(8 * n + 16), lambda b: b[3:3 + n], lambda b: b[n + 8:8 * n + 8].view(7, n)[:, :(n + 1) // 2])
+    return out, backs, masks
+
+
+@pytest.mark.parametrize("count", [7, 60])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("ptype,gtype,master", [(F32, BF16, False), (BF16, BF16, False), (F16, F16, False),
+                                                (BF16, F32, False), (F16, BF16, True), (BF16, F16, True)])
+def test_rows_and_odd_addresses(bits, ptype, gtype, master, count):
+    params, backs, masks = laid_out(1, count, ptype)
+    before = [b.clone() for b in backs]
+    opt = FusedAdamW(params, lr=1e-2, weight_decay=0.1, state_bits=bits, master_weights=master)
+    ref = Reference(opt, params)
+    for s in range(3):
+        grads, _, _ = laid_out(10 + s, count, gtype, scale=1e-2)
+        shapes_differ = [k for k in params if grads[k].shape != params[k].shape]
+        for k in shapes_differ:  # (the small ones' sizes are drawn)
+            grads[k] = torch.randn(params[k].numel() + 1, device=DEV).mul(1e-2).to(gtype)[1:].view(params[k].shape)
+        if s == 1:  # dense gradients of strided parameters
+            grads = {k: g.contiguous() for k, g in grads.items()}
+        opt.step(grads)
+        ref.check(grads, lr=1e-2, master=master)
+    for b, old, mask in zip(backs, before, masks):
+        assert torch.equal(b[~mask], old[~mask])
+
+
+@pytest.mark.parametrize("count", [7, 60])
+@pytest.mark.parametrize("gtype,otype", [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32), (F32, F16), (F16, BF16)])
+def test_clip_rows_and_odd_addresses(gtype, otype, count):
+    grads, _, _ = laid_out(3, count, gtype, scale=0.1)
+    exact = math.sqrt(sum(float(g.double().square().sum()) for g in grads.values()))
+    strided, backs, masks = laid_out(3, count, otype)  # the same shapes
+    before = [b.clone() for b in backs]
+    shifted = {k: torch.empty(g.numel() + 1, dtype=otype, device=DEV)[1:].view(g.shape) for k, g in grads.items()}
+    for out in (strided, shifted, {k: torch.empty(g.shape, dtype=otype, device=DEV) for k, g in grads.items()}):
+        norm = clip_gradients(grads, 0.3 * exact, out=out)
+        assert abs(float(norm) - exact) <= 2.0 ** -24 * 1.01 * exact
+        for k, g in grads.items():
+            want = g.double() * 0.3
+            # two float32 roundings (factor, product) and the type's
+            tol = (HALF_STEP[otype] + 2.0 ** -23 * 1.01) * want.abs() + TINY[otype] + 2.0 ** -149
+            assert ((out[k].double() - want).abs() <= tol).all(), k
+    for b, old, mask in zip(backs, before, masks):
+        assert torch.equal(b[~mask], old[~mask])
+    if gtype == otype:  # in place, the same bits
+        again, backs, masks = laid_out(3, count, gtype, scale=0.1)
+        before = [b.clone() for b in backs]
+        clip_gradients(again, 0.3 * exact)
+        assert all(torch.equal(again[k], strided[k]) for k in grads)
+        for b, old, mask in zip(backs, before, masks):
+            assert torch.equal(b[~mask], old[~mask])
+
+
+@pytest.mark.parametrize("odd", ["m", "v", "both"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("count", [12, 40])
+def test_load_moments_from_odd_addresses(dtype, odd, count, reader):
+    sizes = SIZES + [1 + 37 * i for i in range(count - len(SIZES))]
+    shapes = {f"x{i}": (n,) for i, n in enumerate(sizes)}
+    opt = FusedAdamW(tensors(1, shapes, F32), state_bits=8)
+
+    def shift(x):
+        return torch.cat([x.new_zeros(1), x])[1:]
+
+    m = tensors(2, shapes, dtype, sparse=0.2)
+    v = {k: x.square() for k, x in tensors(3, shapes, dtype, sparse=0.2).items()}
+    if odd != "v":
+        m = {k: shift(x) for k, x in m.items()}
+    if odd != "m":
+        v = {k: shift(x) for k, x in v.items()}
+    opt.load_moments(m, v, t=77)
+    got_m, got_v = opt.moments()
+    for k in shapes:
+        n = m[k].numel()
+        want = oadamw.values(*oadamw.quantize(flat(m[k]), 77, False), False)[:n]
+        np.testing.assert_array_equal(finite(got_m[k]), want, err_msg=k)
+        want = oadamw.values(*oadamw.quantize(flat(v[k]), 77, True), True)[:n]
+        np.testing.assert_array_equal(finite(got_v[k]), want, err_msg=k)
+    live = torch.zeros(opt.slab_elements, dtype=torch.bool, device=DEV)
+    for view in opt._views(live).values():
+        view.fill_(True)
+    assert not opt.m[~live].any() and not opt.v[~live].any()
