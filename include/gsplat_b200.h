@@ -247,7 +247,7 @@ typedef struct gs_adamw_state {
 typedef struct gs_adamw_settings {
     double lr, beta1, beta2;
     float eps;
-    double grad_scale;            /* multiplies every gradient */
+    double grad_scale;            /* multiplies every gradient (finite in float32) */
     const float* lr_device;       /* optional: one float32 on the device that replaces lr */
     const double* norm_partials;  /* optional, from gs_grad_norm_partials over the same gradients: the step clips
                                      them to max_norm (INFINITY: no clipping) and is skipped as a whole, its count

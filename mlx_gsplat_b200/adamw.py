@@ -34,6 +34,7 @@ from . import _lib
 
 TYPES = {torch.float32: _lib.GS_F32, torch.bfloat16: _lib.GS_BF16, torch.float16: _lib.GS_F16}
 BLOCK = _lib.GS_MOMENT_BLOCK
+_F32_MAX = 3.4028234663852886e38
 _ENTRY = np.dtype([("param", np.uint64), ("grad", np.uint64), ("n", np.int64), ("state", np.int64),
                    ("cols", np.int64), ("param_stride", np.int64), ("grad_stride", np.int64),
                    ("param_type", np.int32), ("grad_type", np.int32), ("lr_scale", np.float64),
@@ -402,8 +403,8 @@ class FusedAdamW:
         if grads is not None and not isinstance(grads, Mapping):
             raise TypeError(f"gradients are given by name, not as {type(grads).__name__}")
         grad_scale = float(grad_scale)
-        if not math.isfinite(grad_scale):
-            raise ValueError(f"grad_scale must be finite: {grad_scale}")
+        if not abs(grad_scale) <= _F32_MAX:
+            raise ValueError(f"grad_scale must be finite in float32: {grad_scale}")
         lr, lr_device = self._lr_value()
         limit = self._norm_limit()
         names, shapes, params, entries, on = self.names, self._shapes, self._params, self._entries, None

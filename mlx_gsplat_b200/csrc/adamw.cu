@@ -531,7 +531,7 @@ extern "C" int gs_adamw_step(const gs_tensor* tensors, int64_t count, const gs_a
     GS_REQUIRE(set->beta1 >= 0.0 && set->beta1 < 1.0 && set->beta2 >= 0.0 && set->beta2 < 1.0,
                "adamw: betas must be in [0, 1)");
     GS_REQUIRE(set->eps >= FLT_MIN && isfinite(set->eps), "adamw: eps must be positive (a normal float32)");
-    GS_REQUIRE(isfinite(set->grad_scale), "adamw: grad_scale must be finite");
+    GS_REQUIRE(isfinite((float)set->grad_scale), "adamw: grad_scale must be finite in float32");
     GS_REQUIRE(set->lr_device || isfinite(set->lr), "adamw: lr must be finite");
     GS_REQUIRE(!set->norm_partials || (set->num_partials >= 0 && set->max_norm > 0.0),
                "adamw: clipping needs a partial count and a positive max_norm");

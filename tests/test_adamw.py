@@ -350,6 +350,14 @@ def test_native_reader_writes_no_lazy_copy():
 
 
 @built
+def test_grad_scale_is_a_float32():
+    lib, e = _lib.load(), _entry()
+    for scale in (1e39, -1e39):
+        st = lib.gs_adamw_step(e.ctypes.data, 1, _state(), _settings(grad_scale=scale), None)
+        assert st == _lib.GS_ERR_INVALID and b"grad_scale" in lib.gs_last_error()
+
+
+@built
 def test_counted_calls_pass_over_null_gradients():
     lib = _lib.load()
     e, state = _entry(grad=0), _state()

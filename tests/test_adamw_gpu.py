@@ -1084,3 +1084,19 @@ def test_load_moments_from_odd_addresses(dtype, odd, count, reader):
     for view in opt._views(live).values():
         view.fill_(True)
     assert not opt.m[~live].any() and not opt.v[~live].any()
+
+
+# ---------------------------------------------------------------- settings and state
+def test_grad_scale_beyond_float32(reader):
+    """The kernels hold the scale in float32: one that is infinite there is refused."""
+    params = tensors(1, {"a": (300,)}, F32)
+    before = params["a"].clone()
+    g = tensors(2, {"a": (300,)}, F32, scale=1e-30)
+    opt = FusedAdamW(params)
+    for scale in (1e39, -1e39, 3.5e38):
+        with pytest.raises(ValueError, match="grad_scale"):
+            opt.step(g, grad_scale=scale)
+    assert opt.t == 0 and torch.equal(params["a"], before)
+    ref = Reference(opt, params)
+    opt.step(g, grad_scale=3e38)
+    ref.check(g, scale=3e38)
