@@ -514,7 +514,8 @@ class FusedAdamW:
             else:
                 self._set_steps(t)
             if self.state_bits == 32:
-                torch._foreach_copy_(list(self._views(self.m).values()) + list(self._views(self.v).values()), ml + vl)
+                torch._foreach_copy_(list(self._views(self.m).values()) + list(self._views(self.v).values()),
+                                     [x.detach() for x in ml + vl])
                 return
             lib = _lib.lib()
             _lib.check(lib.gs_moments8_quantize(entries.ctypes.data, len(entries), self.m.data_ptr(),

@@ -1100,3 +1100,16 @@ def test_grad_scale_beyond_float32(reader):
     ref = Reference(opt, params)
     opt.step(g, grad_scale=3e38)
     ref.check(g, scale=3e38)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_loaded_moments_keep_no_autograd_graph(bits):
+    params = tensors(1, {"a": (300,)}, F32)
+    opt = FusedAdamW(params, state_bits=bits)
+    m = torch.randn(300, device=DEV, requires_grad=True)
+    opt.load_moments({"a": m * 2}, {"a": (m * 3).square()}, t=1)
+    assert not opt.m.requires_grad and not opt.v.requires_grad
+    if bits == 32:
+        assert torch.equal(opt.m[:300], (m * 2).detach())
+    opt.t = 2
+    opt.load_state_dict(opt.state_dict())
