@@ -439,3 +439,68 @@ def test_build_does_without_the_helper(tmp_path, monkeypatch, capsys):
     assert not path.exists() and "read in Python" in capsys.readouterr().err
     monkeypatch.setenv("CXX", str(tmp_path / "no such compiler"))
     assert build.build() == build.LIB
+
+
+# ---------------------------------------------------------------- where the 8-bit form ends
+@pytest.mark.parametrize("size", [2.0 ** -3, 2.0 ** -20 * 1.3, 2.0 ** -29 * 1.7, 2.0 ** -32 * 1.1, 2.0 ** -33, 2.0 ** -33 * 0.99,
+                                  2.0 ** -35, 2.0 ** -60])
+def test_v_ends_at_a_step(size):
+    """Beside a largest value of 1 the lowest step is 2^-33.  From there up the mean of
+    the roundings lies within the discrepancy bound (see above) of the value; what
+    is below, and not 0, is held as that step: too large."""
+    x = np.full(256, size, np.float32)
+    x[0] = 1.0
+    n = 1000
+    got = np.array([oadamw.values(*oadamw.quantize(x, t, True), True) for t in range(n)], np.float64)
+    assert (got[:, 0] == 1.0).all()
+    if size < 2.0 ** -33:
+        assert (got[:, 1:] == 2.0 ** -33).all()
+        return
+    d = (3 + (1 / np.log((1 + 5 ** 0.5) / 2) + 2 / np.log(3)) * np.log(n)) / n
+    step = max(2.0 ** (math.frexp(size)[1] - 4), 2.0 ** -33)
+    assert (np.abs(got[:, 1:].mean(0) - float(np.float32(size))) <= (d + 2.0 ** -20) * step).all()
+
+
+def test_v_of_small_gradients_stays_at_the_step():
+    """Elements whose gradients stay below 2^-16.5 of the block's largest: their v
+    is one step, 2^-33 of the block's, however small they are, and with no
+    gradient at all it does not return to 0.  (beta2 = 1/2 keeps the largest at
+    1; a v of one step and a square below it have a mean below it, which is
+    rounded to one step or to 0, and a positive v is never 0.)"""
+    g = np.zeros(256, np.float32)
+    g[0], g[1:100], g[100:200] = 1.0, 2.0 ** -17, 2.0 ** -30
+    v = np.zeros(256, np.float32)
+    v[0] = 1.0
+    v[200:250] = 2.0 ** -33
+    for t in range(200):
+        v = oadamw.values(*oadamw.quantize(np.float32(0.5) * v + np.float32(0.5) * (g * g), t, True), True)
+        assert v[0] == 1.0 and (v[1:250] == 2.0 ** -33).all() and (v[250:] == 0.0).all()
+
+
+@pytest.mark.parametrize("positive", [False, True], ids=["m", "v"])
+def test_grids_are_nested_downward(positive):
+    """Where the block's largest value falls, what the form held is kept exactly; where
+    it rises, values below the new lowest whole binade are rounded again, by
+    less than the new step, and no others."""
+    top = oadamw.V_TOP if positive else oadamw.M_TOP
+    codes = np.arange(256, dtype=np.uint8)
+    if not positive:
+        codes[128:] = 0
+    held = oadamw.values(codes, np.array([127], np.uint8), positive)
+    held[-1] = 1.0  # the largest of these is below 2, and one at least keeps the exponent
+    for t in (0, 5, 77):
+        lower = held.copy()
+        lower[lower >= 2.0 ** -4] = 0.0
+        lower[-1] = 2.0 ** -5  # the exponent falls by five
+        c, e = oadamw.quantize(lower, t, positive)
+        assert e[0] == 122
+        np.testing.assert_array_equal(oadamw.values(c, e, positive), lower)
+        higher = held.copy()
+        higher[-1] = 4.0  # and rises by two
+        c, e = oadamw.quantize(higher, t, positive)
+        assert e[0] == 129
+        got = oadamw.values(c, e, positive)
+        lowest = 2.0 ** (2 - (top - 1))
+        np.testing.assert_array_equal(got[higher >= lowest], higher[higher >= lowest])
+        assert (np.abs(got - higher) < lowest / 8).all()
+        assert (got != higher).any()
