@@ -270,7 +270,7 @@ typedef struct gs_adamw_settings {
 int gs_adamw_step(const gs_tensor* tensors, int64_t count, const gs_adamw_state* state,
                   const gs_adamw_settings* settings, gs_stream_t stream);
 
-/* Partial sums, in float64, of the squares of every tensor's ``grad``; their
+/* Partial sums, in float64, of the squares of every tensor's ``grad`` (null: none); their
  * number, at most gs_grad_norm_max_partials(count), is returned through the
  * host pointer ``num_partials``. */
 int64_t gs_grad_norm_max_partials(int64_t count);

@@ -194,13 +194,16 @@ def load_tensors(path: str) -> ctypes.PyDLL:
         abi = dll.gst_abi().decode()
     except AttributeError:
         abi = "an unknown torch"
-    if not all(hasattr(dll, name) for name in ("gst_fill", "gst_params_unmoved", "gst_clip")):
+    if not all(hasattr(dll, name) for name in ("gst_fill", "gst_step", "gst_params_unmoved", "gst_params_as_taken",
+                                                "gst_clip")):
         raise OSError(f"{path} is not the tensor helper")
     if abi != tensors_abi():
         raise OSError(f"{path} was compiled against {abi}, not {tensors_abi()}")
     obj, size = ctypes.py_object, ctypes.c_ssize_t
     dll.gst_fill.argtypes = [obj, obj, obj, obj, c_vp, size, ctypes.c_int]
+    dll.gst_step.argtypes = [obj, obj, obj, obj, c_vp, size, ctypes.c_int, ctypes.POINTER(size)]
     dll.gst_params_unmoved.argtypes = [obj, c_vp, size]
+    dll.gst_params_as_taken.argtypes = [obj, obj, c_vp, size]
     dll.gst_clip.argtypes = [obj, obj, c_vp, size, ctypes.POINTER(ctypes.c_int)]
     return dll
 

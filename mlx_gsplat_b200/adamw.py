@@ -149,6 +149,10 @@ class _on_device:
             torch.cuda.set_device(self.prev)
 
 
+def _copied(entries: np.ndarray) -> np.ndarray:
+    return entries.view(np.uint8).copy().view(_ENTRY)  # (a copy of bytes: field by field it takes 7 us)
+
+
 def _changed(tensors: List[torch.Tensor]) -> None:
     """Tells autograd that the tensors were written."""
     try:
@@ -264,6 +268,7 @@ class FusedAdamW:
         self._control = torch.zeros(2 + n, dtype=torch.int64, device=self.device)
         self._count, self._missed = self._control[0], self._control[2:]
         self._any_missed = False  # whether any call so far left a parameter out
+        self._found = (ctypes.c_ssize_t * 2)()
         self.master_slab: Optional[torch.Tensor] = None
         if master_weights and any(p.dtype != torch.float32 for p in self._params):
             self.master_slab = torch.zeros(self.slab_elements, dtype=torch.float32, device=self.device)
@@ -325,6 +330,9 @@ class FusedAdamW:
     def _as_taken(self) -> bool:
         """Whether the parameters are the memory, types and layouts of the entries."""
         ps = self._params
+        native = _lib.tensors()
+        if native is not None:
+            return not native.gst_params_as_taken(ps, self._aliases, self._at, len(ps))
         return list(map(_data_ptr, ps)) == self._ptrs and list(map(_dtype, ps)) == self._types and \
             list(map(_shape, ps)) == self._shapes and list(map(_stride, ps)) == self._strides and \
             not any(map(_is_neg, ps))
@@ -359,7 +367,7 @@ class FusedAdamW:
             same = list(map(_shape, grads)) == shapes
             here = set(map(_device_index, grads)) == {self.device.index}
             dense = all(map(_is_contiguous, grads))
-            entries["grad"] = list(map(_data_ptr, grads))
+            entries["grad"] = ptrs = list(map(_data_ptr, grads))
         except (KeyError, AttributeError, TypeError, RuntimeError):
             for name, g in zip(names, grads):
                 _check_tensor(f"{what} of {name!r}", g)
@@ -370,7 +378,7 @@ class FusedAdamW:
                     raise ValueError(f"{what} of {name!r} has shape {tuple(g.shape)}, not {tuple(s)}")
         if not here:
             raise ValueError(f"every {what} must be on {self.device}")
-        if ((entries["grad"] == 0) & (entries["n"] > 0)).any():
+        if 0 in ptrs and ((entries["grad"] == 0) & (entries["n"] > 0)).any():
             raise ValueError(f"a {what} has no memory")
         entries["grad_type"] = codes
         entries["grad_stride"] = entries["cols"]
@@ -409,11 +417,13 @@ class FusedAdamW:
         limit = self._norm_limit()
         names, shapes, params, entries, on = self.names, self._shapes, self._params, self._entries, None
         native = _lib.tensors()
-        # every gradient there, dense and as expected: the table is filled natively
-        filled = native is not None and \
-            not native.gst_fill(grads, names, params, self._aliases, self._at, len(params), self.device.index) and \
-            not native.gst_params_unmoved(params, self._at, len(params))
-        if not filled:
+        # gradients dense and as expected, or missing: the table is filled natively
+        filled = native is not None and not native.gst_step(grads, names, params, self._aliases, self._at, len(params),
+                                                            self.device.index, self._found)
+        if filled:
+            elements = self._found[1] != 0
+            self._any_missed |= self._found[0] != len(params)
+        else:
             if grads is None:
                 found = [p.grad for p in params]
             else:
@@ -428,12 +438,13 @@ class FusedAdamW:
                 on = [k for k, g in enumerate(found) if g is not None]
                 entries = entries[on]
                 names, shapes, params, found = ([x[k] for k in on] for x in (names, shapes, params, found))
+            elements = self._elements_in(entries)
         with_norm = self.max_norm is not None or self.skip_nonfinite
         norm = None
         with _on_device(self.device):
             if with_norm:
                 norm = torch.empty((), dtype=torch.float32, device=self.device)
-            if not self._elements_in(entries):
+            if not elements:
                 return norm.zero_() if with_norm else None
             if not filled:
                 entries, keep = self._with_grads(entries, names, shapes, found)
@@ -446,7 +457,7 @@ class FusedAdamW:
                 s.norm_partials = buffer.data_ptr()
                 s.norm_out = norm.data_ptr()
             if on is not None:  # the step takes the whole list, those that miss it without a gradient
-                every = self._entries.copy()
+                every = _copied(self._entries)
                 every["grad"] = 0
                 every[on] = entries
                 at, count, self._any_missed = every.ctypes.data, len(every), True
@@ -503,7 +514,7 @@ class FusedAdamW:
             raise ValueError(f"the step count must not be negative: {t}")
         ml, vl = list(map(m.__getitem__, self.names)), list(map(v.__getitem__, self.names))
         with _on_device(self.device):
-            entries = self._entries.view(np.uint8).copy().view(_ENTRY)  # (a copy of bytes: field by field it takes 7 us)
+            entries = _copied(self._entries)
             entries["cols"] = entries["param_stride"] = np.maximum(entries["n"], 1)
             # a tensor's first place takes its m, the second its v
             ml = self._fill_dense(entries, ml, "moment m")

@@ -196,7 +196,7 @@ extern "C" int gs_grad_norm_partials(const gs_tensor* tensors, int64_t count, do
     GS_REQUIRE(num_partials, "grad_norm: null count");
     *num_partials = 0;
     int64_t live;
-    GS_TRY(check_tensors("grad_norm", tensors, count, kNeedGrad, live));
+    GS_TRY(check_tensors("grad_norm", tensors, count, kNeedGrad | kMayMiss, live));
     if (live == 0) return GS_OK;
     GS_REQUIRE(partials && capacity > 0, "grad_norm: null partial sums");
     const cudaStream_t st = (cudaStream_t)stream;

@@ -48,6 +48,58 @@ void changed(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// See gst_fill.  ``may_miss``: a name that the dict lacks or that has None, or a parameter
+// without ``grad``, has a null one; ``present`` counts the others.
+bool fill(PyObject* items, PyObject* names, PyObject* owners, PyObject* like, gs_tensor* e, Py_ssize_t n, int device,
+          bool may_miss, Py_ssize_t& present) {
+    present = 0;
+    try {
+        const bool list = PyList_Check(items), dict = PyDict_Check(items);
+        if (!(list || dict || items == Py_None) || !PyList_Check(like) || PyList_GET_SIZE(like) != n ||
+            (list && PyList_GET_SIZE(items) != n) ||
+            (dict && ((!may_miss && PyDict_GET_SIZE(items) != n) || !PyList_Check(names) ||
+                      PyList_GET_SIZE(names) != n)) ||
+            (items == Py_None && owners == Py_None) ||
+            (owners != Py_None && (!PyList_Check(owners) || PyList_GET_SIZE(owners) != n)))
+            return false;
+        Py_ssize_t named = 0;
+        for (Py_ssize_t k = 0; k < n; ++k) {
+            const at::Tensor* p = tensor_of(PyList_GET_ITEM(like, k));
+            if (!p) return false;
+            const at::Tensor *g = nullptr, *owner = nullptr;
+            if (owners != Py_None && (!(owner = tensor_of(PyList_GET_ITEM(owners, k))) || !same_form(*owner, *p)))
+                return false;
+            bool none = false;
+            if (list) {
+                g = tensor_of(PyList_GET_ITEM(items, k));
+            } else if (dict) {
+                PyObject* item = PyDict_GetItem(items, PyList_GET_ITEM(names, k));
+                named += item != nullptr;
+                none = !item || item == Py_None;
+                g = tensor_of(item);
+            } else {
+                g = &owner->grad();
+                none = !g->defined();
+            }
+            if (none && may_miss) {
+                e[k].grad = nullptr;
+                continue;
+            }
+            if (!g) return false;
+            const int type = dense_type(*g, device);
+            if (type < 0 || g->sizes() != p->sizes()) return false;
+            e[k].grad = g->const_data_ptr();
+            if (!e[k].grad && g->numel() > 0) return false;
+            e[k].grad_type = type;
+            e[k].grad_stride = e[k].cols;
+            ++present;
+        }
+        return !dict || named == PyDict_GET_SIZE(items);
+    } catch (...) {
+        return false;
+    }
+}
+
 struct Span {
     uintptr_t lo, hi;
     bool operator<(const Span& o) const { return lo < o.lo; }
@@ -64,38 +116,8 @@ extern "C" const char* gst_abi() { return GST_ABI; }
 // given, must still have the form of ``like``.
 extern "C" int gst_fill(PyObject* items, PyObject* names, PyObject* owners, PyObject* like, gs_tensor* e, Py_ssize_t n,
                         int device) {
-    try {
-        const bool list = PyList_Check(items), dict = PyDict_Check(items);
-        if (!(list || dict || items == Py_None) || !PyList_Check(like) || PyList_GET_SIZE(like) != n ||
-            (list && PyList_GET_SIZE(items) != n) ||
-            (dict && (PyDict_GET_SIZE(items) != n || !PyList_Check(names) || PyList_GET_SIZE(names) != n)) ||
-            (items == Py_None && owners == Py_None) ||
-            (owners != Py_None && (!PyList_Check(owners) || PyList_GET_SIZE(owners) != n)))
-            return 1;
-        for (Py_ssize_t k = 0; k < n; ++k) {
-            const at::Tensor* p = tensor_of(PyList_GET_ITEM(like, k));
-            if (!p) return 1;
-            const at::Tensor *g = nullptr, *owner = nullptr;
-            if (owners != Py_None && (!(owner = tensor_of(PyList_GET_ITEM(owners, k))) || !same_form(*owner, *p)))
-                return 1;
-            if (list)
-                g = tensor_of(PyList_GET_ITEM(items, k));
-            else if (dict)
-                g = tensor_of(PyDict_GetItem(items, PyList_GET_ITEM(names, k)));
-            else
-                g = &owner->grad();
-            if (!g) return 1;
-            const int type = dense_type(*g, device);
-            if (type < 0 || g->sizes() != p->sizes()) return 1;
-            e[k].grad = g->const_data_ptr();
-            if (!e[k].grad && g->numel() > 0) return 1;
-            e[k].grad_type = type;
-            e[k].grad_stride = e[k].cols;
-        }
-        return 0;
-    } catch (...) {
-        return 1;
-    }
+    Py_ssize_t present;
+    return fill(items, names, owners, like, e, n, device, false, present) ? 0 : 1;
 }
 
 // Whether the parameters still lie where the entries say, and if so tells autograd
@@ -109,6 +131,42 @@ extern "C" int gst_params_unmoved(PyObject* params, const gs_tensor* e, Py_ssize
             if (!p || p->mutable_data_ptr() != e[k].param) return 1;
         }
         for (Py_ssize_t k = 0; k < n; ++k) changed(THPVariable_Unpack(PyList_GET_ITEM(params, k)));
+        return 0;
+    } catch (...) {
+        return 1;
+    }
+}
+
+// A step's entries: gradients as gst_fill takes them, where any may be missing, for
+// parameters that still are where the entries say, which are then told to be
+// written.  ``found``: the gradients that are there, and whether they have any element.
+extern "C" int gst_step(PyObject* grads, PyObject* names, PyObject* params, PyObject* like, gs_tensor* e, Py_ssize_t n,
+                        int device, Py_ssize_t* found) {
+    if (params == Py_None || PyList_Check(grads) || !fill(grads, names, params, like, e, n, device, true, found[0])) return 1;
+    found[1] = 0;
+    for (Py_ssize_t k = 0; k < n; ++k) found[1] |= e[k].grad && e[k].n;
+    if (found[0] == n) return gst_params_unmoved(params, e, n);
+    try {
+        for (Py_ssize_t k = 0; k < n; ++k)
+            if (THPVariable_Unpack(PyList_GET_ITEM(params, k)).mutable_data_ptr() != e[k].param) return 1;
+        for (Py_ssize_t k = 0; k < n; ++k)
+            if (e[k].grad) changed(THPVariable_Unpack(PyList_GET_ITEM(params, k)));
+        return 0;
+    } catch (...) {
+        return 1;
+    }
+}
+
+// Whether the parameters are the memory, types and layouts that the entries and
+// ``like`` were taken from.
+extern "C" int gst_params_as_taken(PyObject* params, PyObject* like, const gs_tensor* e, Py_ssize_t n) {
+    try {
+        if (!PyList_Check(params) || PyList_GET_SIZE(params) != n || !PyList_Check(like) || PyList_GET_SIZE(like) != n)
+            return 1;
+        for (Py_ssize_t k = 0; k < n; ++k) {
+            const at::Tensor *p = tensor_of(PyList_GET_ITEM(params, k)), *was = tensor_of(PyList_GET_ITEM(like, k));
+            if (!p || !was || p->mutable_data_ptr() != e[k].param || !same_form(*p, *was)) return 1;
+        }
         return 0;
     } catch (...) {
         return 1;

@@ -367,7 +367,9 @@ def test_counted_calls_pass_over_null_gradients():
     state.counted = 2
     assert lib.gs_adamw_step(e.ctypes.data, 1, state, _settings(), None) == _lib.GS_ERR_INVALID
     assert b"counted" in lib.gs_last_error()
-    assert lib.gs_grad_norm_partials(e.ctypes.data, 1, 4096, 8, ctypes.byref(ctypes.c_int64()), None) == _lib.GS_ERR_INVALID
+    got = ctypes.c_int64(7)
+    assert lib.gs_grad_norm_partials(e.ctypes.data, 1, 4096, 8, ctypes.byref(got), None) == 0 and got.value == 0
+    assert lib.gs_clip_gradients(e.ctypes.data, 1, 4096, 1, 1.0, None, None) == _lib.GS_ERR_INVALID
 
 
 # ---------------------------------------------------------------- the native reader's library

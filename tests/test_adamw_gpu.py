@@ -1113,3 +1113,20 @@ def test_loaded_moments_keep_no_autograd_graph(bits):
         assert torch.equal(opt.m[:300], (m * 2).detach())
     opt.t = 2
     opt.load_state_dict(opt.state_dict())
+
+
+def test_parameters_that_miss_a_step_are_not_marked_as_written(reader):
+    params = {k: torch.randn(20, device=DEV, requires_grad=True) for k in "abc"}
+    opt = FusedAdamW(params)
+    versions = {k: p._version for k, p in params.items()}
+    opt.step({"a": torch.ones(20, device=DEV), "b": None})
+    params["c"].grad = torch.ones(20, device=DEV)
+    opt.step()
+    assert params["a"]._version > versions["a"] and params["c"]._version > versions["c"]
+    assert params["b"]._version == versions["b"] and opt.t == 2
+    assert opt.step({}) is None and opt.step({"a": None}) is None and opt.t == 2
+    with pytest.raises(ValueError, match="no parameter named"):
+        opt.step({"a": torch.ones(20, device=DEV), "z": torch.ones(20, device=DEV)})
+    with pytest.raises(ValueError, match="no parameter named"):
+        opt.step({"z": None})
+    assert opt.t == 2
