@@ -10,11 +10,14 @@ all sizes instead.  ``FusedAdamW`` steps all of them in one launch:
 * parameters and gradients in float32, bfloat16 or float16, optionally with
   float32 master copies of the 16-bit parameters;
 * moments in 32 bits, or in 8 (``state_bits=8``: 2.02 bytes a parameter instead
-  of 8), rounded without bias over steps, ``moments8.cuh``;
+  of 8): 256 neighbours share a scale, and values are rounded without bias over
+  steps.  Gradients below 1.1e-5 of the largest among the 256 are damped: their
+  second moment has reached the form's lowest step (``moments8.cuh``);
 * clipping by the global gradient norm inside the step (``max_norm``), and
   skipping of a step whose gradients are not all finite, without a host sync;
-* the step count on the device, so that ``step`` can be captured into a CUDA
-  graph and replayed (``lr`` may be a device tensor).
+* the step counts on the device, so that ``step`` can be captured into a CUDA
+  graph and replayed (``lr`` may be a device tensor; ``grad_scale`` is a number
+  of the host, fixed in a graph).
 
 ``clip_gradients`` clips a set of gradients on its own, for other optimizers.
 """
@@ -183,8 +186,10 @@ class FusedAdamW:
     factors of ``lr`` and ``weight_decay`` (1 where a name is missing).
     ``state_bits``: 32 or 8.  ``master_weights``: keep float32 copies of the
     16-bit parameters and round the parameters from them (call
-    ``sync_master`` after changing such parameters elsewhere).  ``max_norm``:
-    clip the gradients to this global norm inside the step.
+    ``sync_master`` after changing such parameters elsewhere; the slab of
+    copies has room for every parameter, 4 bytes an element, also where only
+    some have 16 bits).  ``max_norm``: clip the gradients to this global norm
+    inside the step.
     ``skip_nonfinite``: leave parameters, moments and the step count as they
     are when a gradient is not finite (a step with ``max_norm`` always does).
 
@@ -192,7 +197,9 @@ class FusedAdamW:
     does not count the step: its bias corrections are those of the steps that
     it took itself.
 
-    Parameters may be strided rows (a pool's columns); they may not overlap.
+    Parameters may be strided rows (a pool's columns) but not permuted ones
+    (transposed, channels last); they may not overlap, and gradients may not
+    lie in their memory.
     ``lr``, ``weight_decay``, ``beta1``, ``beta2``, ``eps``, ``max_norm`` and
     ``skip_nonfinite`` may be changed between steps (a captured step keeps the
     values it was captured with, but for a tensor ``lr``).  The optimizer
@@ -403,10 +410,11 @@ class FusedAdamW:
     def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_scale: float = 1.0) -> Optional[torch.Tensor]:
         """One step on the current stream.  ``grads``: name -> gradient (default:
         the parameters' ``.grad``); a parameter without one keeps its values and
-        moments and misses the step, and a step without any does nothing.  ``grad_scale`` multiplies
-        every gradient first (the inverse of a loss scale).  Returns the global
-        norm of the scaled gradients before clipping as a device scalar when
-        ``max_norm`` or ``skip_nonfinite`` asks for it, else None."""
+        moments and misses the step, and a step without any does nothing.
+        ``grad_scale`` multiplies every gradient first (the inverse of a loss
+        scale).  Returns the global norm of the scaled gradients before clipping
+        as a device scalar when ``max_norm`` or ``skip_nonfinite`` asks for it,
+        else None."""
         lib = _lib.lib()
         if grads is not None and not isinstance(grads, Mapping):
             raise TypeError(f"gradients are given by name, not as {type(grads).__name__}")

@@ -14,7 +14,7 @@
 //
 // A step moves 28 bytes a float32 parameter with 32-bit moments and 16 with 8-bit
 // ones.  59M parameters (of measured copy rate, 6.55 TB/s): 256 us (98 %) and 153 us
-// (94 %); with 8-bit moments the 53 instructions an element take 60 % of the issue
+// (94 %); with 8-bit moments the 52 instructions an element take 59 % of the issue
 // slots, so both bounds are near.  Quantizing them takes 97 us (93 %), reading them
 // back as bfloat16 56 us (96 %).
 #include <float.h>
@@ -30,12 +30,15 @@ namespace gs {
 // threads already have enough in flight; three are slower, since more reads and
 // writes at once disturb one another in DRAM (59M parameters: 256 us with two, 297
 // with three), and single chunks keep the blocks closest together (272 us with 16).  8-bit moments:
-// nearly as much arithmetic as memory time, so the registers' most, three; groups
-// as large as the exponents' (moments8.cuh) and no larger.
+// nearly as much arithmetic as memory time, so the registers' most, three; groups of
+// half the chunks whose exponents a warp can hold (moments8.cuh).
 // Where a tensor of the call has rows or odd alignment, its single accesses wait
-// longer and one more block per SM is better (columns of a pool of 1M Gaussians: 481
-// us with three, 516 with two; 8-bit moments 414 with four, 443 with three), which is
-// why such calls have kernels of their own.
+// longer and one more block per SM is better, which is why such calls have kernels of
+// their own.  Columns of a pool of 1M Gaussians, dense gradients: 489 us with three,
+// 520 with two; 8-bit moments 421 with four, 449 with three (strided gradients: 636
+// and 655; 598 and 629).  Dense float32 parameters at odd addresses: 295 us with three,
+// 346 with two; but with 8-bit moments 352 with four and 337 with three, which the
+// columns outweigh.
 constexpr int kBlocks32 = 2, kBlocks32Rows = 3, kGroup32 = 1;
 constexpr int kBlocks8 = 3, kBlocks8Rows = 4, kGroup8 = 16;
 constexpr int kBlocksQuantize = 4, kBlocksQuantizeRows = 3;

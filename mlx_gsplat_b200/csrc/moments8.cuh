@@ -6,8 +6,10 @@
 // mantissa bits.  An exponent field f >= 1 (top field T = 15 for m, 31 for v)
 // over mantissa bits q stands for 2^(e - 127 - T + f) (1 + q / 8), field 0 for
 // q times the step of field 1.  The block's scale is a power of two, so the
-// grids of different e are nested: a value on the grid stays on it when e moves,
-// and a block whose values do not change is written back unchanged.
+// grids of different e are nested: a value on the grid stays on it when e falls,
+// and a block whose values do not change is written back unchanged.  When e rises,
+// the values below the new field 1 (2^-14 of the block's binade for m, 2^-30 for v)
+// are rounded again, to the new step there.
 //
 // Rounding adds an offset u in [0, 1) steps and cuts.  To nearest would be wrong
 // here: with beta2 = 0.999 a step moves v by about 0.1 %, less than half of any
@@ -16,7 +18,12 @@
 // sqrt(2), begun at the element's index times the golden ratio, modulo 1), so what
 // a rounding leaves out comes back after a few steps; it needs no state.
 // v's offset is the complement of m's.  A positive v is never rounded to 0, which
-// bounds m / sqrt(v): both forms reach about 2^-17 of the block's largest size.
+// bounds m / sqrt(v): both forms reach about 2^-17 of the block's largest size.  The
+// price: rounding is without bias down to one step, 2^-33 of the block's binade, and
+// below it v is held as that step.  An element whose gradients stay below 2^-16.5
+// (1.1e-5) of the block's largest has too large a v and moves less than it should,
+// the less the smaller they are; without any gradient its v stays at the step.  A
+// value in the last eighth of float32's largest binade may be rounded to infinity.
 //
 // A magnitude is rounded in its float32 bits: bits + u (20 bits) cut to the upper 3
 // mantissa bits is floor(x / step + u) * step for every x of a whole binade, and
