@@ -328,7 +328,8 @@ class FusedAdamW:
         return self._partials
 
     def _take_memory(self) -> None:
-        # aliases keep the memory that the entries point to alive, and its layout, whatever happens to the caller's tensors
+        # aliases keep the memory that the entries point to alive, and its layout, whatever happens to the caller's
+        # tensors
         self._aliases = [p.detach() for p in self._params]
         self._ptrs = list(map(_data_ptr, self._params))
         self._types = list(map(_dtype, self._params))
@@ -514,8 +515,9 @@ class FusedAdamW:
     def load_moments(self, m: Dict[str, torch.Tensor], v: Dict[str, torch.Tensor], t: Optional[int] = None) -> None:
         """Sets every parameter's moments (tensors of the parameters' shapes on
         their device, any of the three types; v must not be negative) and the
-        step count, which is then every parameter's (None: the counts stay).  With 8-bit moments values that the form holds are kept
-        exactly and others are rounded with the step count's offsets."""
+        step count, which is then every parameter's (None: the counts stay).
+        With 8-bit moments values that the form holds are kept exactly and
+        others are rounded with the step count's offsets."""
         if m.keys() != self.offsets.keys() or v.keys() != self.offsets.keys():
             raise ValueError("moments for exactly the optimizer's parameters are needed")
         if t is not None and t < 0:

@@ -79,7 +79,9 @@ __device__ __forceinline__ float inverse_sqrt_correction2(double log2_b2, int64_
 }
 // Called for the further tensors of a block where any missed a step.  In line, this code between the chunks costs
 // every step: a tiny scene in a graph takes 3.6 us instead of 3.4.
-__device__ __noinline__ double further_correction1(double log2_b1, int64_t t) { return inverse_correction1(log2_b1, t); }
+__device__ __noinline__ double further_correction1(double log2_b1, int64_t t) {
+    return inverse_correction1(log2_b1, t);
+}
 __device__ __noinline__ float further_correction2(double log2_b2, int64_t t) {
     return inverse_sqrt_correction2(log2_b2, t);
 }

@@ -142,7 +142,9 @@ extern "C" int gst_params_unmoved(PyObject* params, const gs_tensor* e, Py_ssize
 // written.  ``found``: the gradients that are there, and whether they have any element.
 extern "C" int gst_step(PyObject* grads, PyObject* names, PyObject* params, PyObject* like, gs_tensor* e, Py_ssize_t n,
                         int device, Py_ssize_t* found) {
-    if (params == Py_None || PyList_Check(grads) || !fill(grads, names, params, like, e, n, device, true, found[0])) return 1;
+    if (params == Py_None || PyList_Check(grads) ||
+        !fill(grads, names, params, like, e, n, device, true, found[0]))
+        return 1;
     found[1] = 0;
     for (Py_ssize_t k = 0; k < n; ++k) found[1] |= e[k].grad && e[k].n;
     if (found[0] == n) return gst_params_unmoved(params, e, n);

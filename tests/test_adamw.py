@@ -444,8 +444,8 @@ def test_build_does_without_the_helper(tmp_path, monkeypatch, capsys):
 
 
 # ---------------------------------------------------------------- where the 8-bit form ends
-@pytest.mark.parametrize("size", [2.0 ** -3, 2.0 ** -20 * 1.3, 2.0 ** -29 * 1.7, 2.0 ** -32 * 1.1, 2.0 ** -33, 2.0 ** -33 * 0.99,
-                                  2.0 ** -35, 2.0 ** -60])
+@pytest.mark.parametrize("size", [2.0 ** -3, 2.0 ** -20 * 1.3, 2.0 ** -29 * 1.7, 2.0 ** -32 * 1.1, 2.0 ** -33,
+                                  2.0 ** -33 * 0.99, 2.0 ** -35, 2.0 ** -60])
 def test_v_ends_at_a_step(size):
     """Beside a largest value of 1 the lowest step is 2^-33.  From there up the mean of
     the roundings lies within the discrepancy bound (see above) of the value; what
